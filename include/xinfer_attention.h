@@ -44,7 +44,10 @@ enum {
   XINFER_ERR_ROPE_SHAPE = 15,     /* xinfer_qk_norm_rope_append shapes (no reference message) */
   XINFER_ERR_EPS = 16,            /* RMSNorm epsilon not finite and >= 0 (no reference message) */
   XINFER_ERR_SCRATCH = 17,        /* the call needs more than XINFER_NOALLOC_SCRATCH_BYTES of scratch */
-  XINFER_ERR_CAPTURE_ROWS = 18    /* graph-capture mode: more than 64 rows */
+  XINFER_ERR_CAPTURE_ROWS = 18,   /* graph-capture mode: more than 64 rows */
+  XINFER_ERR_KV4_CACHE = 19,      /* 4-bit cache: head dim, page size, alignment or size */
+  XINFER_ERR_KV4_SHAPE = 20,      /* 4-bit cache: tensors that do not match it or each other */
+  XINFER_ERR_PAGES = 21           /* page tables: page size, table width or ring size */
 };
 
 /* A strided rank-4 view of bf16 device memory, [batch, heads, sequence, dim].
@@ -213,6 +216,96 @@ int xinfer_qk_norm_rope_append(const xinfer_view4 *q, const xinfer_view4 *key, c
 enum { XINFER_BF16 = 0, XINFER_FP32 = 1 };
 int xinfer_projection_gemv(const void *x, const void *weight, void *out, int64_t n, int64_t k, int dtype,
                            void *stream);
+
+/* ---------------------------------------------------------------------------
+ * Paged 4-bit KV cache.  No reference counterpart: the reference holds bf16
+ * caches of one page per row.
+ *
+ * A key or value vector is held as blocks of 32 features.  A feature takes
+ * four bits, e2m1: a sign and a magnitude of 0, 0.5, 1, 1.5, 2, 3, 4 or 6, the
+ * even feature in a byte's low half; a block has one scale byte s, for
+ * 2^(s - 127).  A block whose largest magnitude is a has
+ * s - 127 = e = floor(log2 a) - 2, one more where a > 7 * 2^e, kept in
+ * [-125, 125]; a feature takes the value nearest to it, ties to the even code.
+ * A token whose key or value has an infinity or a NaN holds zeros, and 255 in
+ * all of its key's scales: queries that see it get NaN.  Value scales above
+ * 252 (which no call writes) are read as 252.
+ *
+ * Pages of `page_size` tokens (64, 128 or 256): codes uint8
+ * [pages][kv_heads][page_size][dim / 2], scales uint8
+ * [pages][kv_heads][dim / 32][page_size], key and value apart, 16-byte
+ * aligned; dim in {64, 128, 256}.  A slot is page * page_size + place.
+ * ------------------------------------------------------------------------- */
+typedef struct xinfer_kv4_cache {
+  void *key, *key_scale, *value, *value_scale;
+  int64_t pages, kv_heads, page_size, dim;
+} xinfer_kv4_cache;
+
+/* Pages, slots and positions of a step from the rows' lengths, on the device.
+ * Row r held ceil(kv_before[r] / P) pages and is to hold ceil(kv_lengths[r] / P),
+ * with its last query_lengths[r] tokens new.  free_pages is a ring: entries
+ * counters[0] <= i < counters[1] (modulo ring_size) are free.  Growing rows take
+ * pages from its head in row order into block_table [rows][table_width];
+ * shrinking rows (an ended request has length 0) put theirs at its tail, for
+ * later calls.  A row whose pages, with those of the rows before it, exceed the
+ * free ones, or that does not fit its table row, keeps its pages and takes no part:
+ * lengths[0][r] (new tokens) is 0 and lengths[1][r] is kv_before[r]; otherwise
+ * they are query_lengths[r] and kv_lengths[r].  positions and slots [rows][tokens]
+ * are written whole: of token t < lengths[0][r] the position kv_lengths[r] -
+ * query_lengths[r] + t and its slot, else 0 and -1.  new_counters receives the
+ * ring's head and tail; it must not be counters.  The same inputs give the same
+ * results again.  Out-of-range lengths are clamped ([0, tokens] new tokens,
+ * lengths of at least that), so no input reaches outside the arrays.
+ * table_width * page_size and rows * table_width stay below 2^31. */
+int xinfer_paged_kv_reserve(const int32_t *kv_before, const int32_t *kv_lengths, const int32_t *query_lengths,
+                            int64_t rows, int64_t tokens, int64_t page_size, const int64_t *counters,
+                            int32_t *block_table, int64_t table_width, int32_t *free_pages, int64_t ring_size,
+                            int32_t *lengths, int64_t *positions, int64_t *slots, int64_t *new_counters,
+                            void *stream);
+
+/* Quantises key/value [B,Hkv,T,D] (bf16, layout as for attention tensors) into
+ * slots [B,T] (device int64, strides in elements).  Slots outside the cache,
+ * negative ones among them, are skipped.  The slots of one call are distinct; one
+ * given twice holds codes of either token. */
+int xinfer_append_kv4(const xinfer_view4 *key, const xinfer_view4 *value, const int64_t *slots,
+                      int64_t slot_stride_b, int64_t slot_stride_t, const xinfer_kv4_cache *cache, void *stream);
+
+/* What the cache holds at slots [B,T], as bf16 (exact): key and value contiguous
+ * [B,Hkv,T,D], 16-byte aligned, zero for slots outside the cache, NaN for keys of
+ * tokens that were not finite. */
+int xinfer_read_kv4(const xinfer_kv4_cache *cache, const int64_t *slots, int64_t slot_stride_b,
+                    int64_t slot_stride_t, int64_t batch, int64_t tokens, void *key, void *value, void *stream);
+
+/* q/k RMSNorm, rotary embedding and append in one launch.  Per (token, head)
+ * row: y = x * rsqrt(mean(x^2) + eps) * (weight + weight_offset), then the first
+ * R features turn by cos/sin [B,1,T,R] (R = cos->size[3], a multiple of 16 up to D):
+ * y_i cos_i - y_{i+R/2} sin_i for i < R/2, y_i cos_i + y_{i-R/2} sin_i for the
+ * second half.  All in fp32; the query is rounded once into q_out, contiguous
+ * [B,Hq,T,D], for every token; the key is quantised from fp32 and appended with the
+ * value as in xinfer_append_kv4.  weight_offset: 0, or 1 for weights stored minus
+ * one. */
+int xinfer_qk_norm_rope_append_kv4(const xinfer_view4 *q, const xinfer_view4 *key, const xinfer_view4 *value,
+                                   const void *q_weight, const void *k_weight, double eps, double weight_offset,
+                                   const xinfer_view4 *cos, const xinfer_view4 *sin, const int64_t *slots,
+                                   int64_t slot_stride_b, int64_t slot_stride_t, void *q_out,
+                                   const xinfer_kv4_cache *cache, void *stream);
+
+/* Attention over the cache: q [B,Hq,T,D]; row r's first lengths[0][r] queries see
+ * its lengths[1][r] keys, lower-right causal (query i sees keys up to length -
+ * count + i), key p in page block_table[r][p / P].  lengths is DEVICE int32 [2][B],
+ * as xinfer_paged_kv_reserve writes it; the launch depends on the shapes and on
+ * max_length alone, so a captured call serves every set of lengths up to it.
+ * max_length: the host's bound on the rows' lengths (0: the table's
+ * capacity); longer rows are read as max_length keys.  With M the smaller of
+ * the two, counts are clamped to [0, min(T, M)] and lengths to [count, M].  Keys of table
+ * entries outside the cache count as absent.  out: contiguous bf16 [B,T,Hq,D], zero
+ * for padded queries and for queries that see no key.  The workspace is 16-byte
+ * aligned and serves one call at a time. */
+size_t xinfer_paged_attention_kv4_workspace_size(const xinfer_view4 *q, const xinfer_kv4_cache *cache,
+                                                 int64_t table_width, int64_t max_length);
+int xinfer_paged_attention_kv4(const xinfer_view4 *q, const xinfer_kv4_cache *cache, const int32_t *block_table,
+                               int64_t table_width, const int32_t *lengths, int64_t max_length, double scale,
+                               void *out, void *workspace, size_t workspace_bytes, void *stream);
 
 /* The AOTInductor C shims of the same library are declared in
  * xinfer_attention_aoti.h. */

@@ -20,7 +20,10 @@ which registers these operators in the `xinfer` namespace:
   of the reference's Triton op (compiler/common/kernels/projection_gemv.py);
 * ``qk_norm_rope_append`` -- the step before the attention operator in one
   launch: q/k RMSNorm, rotary embedding and the KV append
-  (compiler/qwen3/adapters/attention.py:44-51), see xinfer_amd/norm_rope.py.
+  (compiler/qwen3/adapters/attention.py:44-51), see xinfer_amd/norm_rope.py;
+* ``paged_kv_reserve``, ``append_kv4``, ``read_kv4``, ``qk_norm_rope_append_kv4``
+  and ``paged_attention_kv4`` -- a paged KV cache held in 4 bits, see
+  xinfer_amd/paged_kv4.py.
 """
 
 import os
@@ -219,6 +222,11 @@ def load_attention_ops(library=None, *, model=None):
             torch._check(q_weight.shape == (q.shape[3],) and k_weight.shape == q_weight.shape)
             torch._check(cache_key.is_contiguous() and cache_value.is_contiguous())
             return q.new_empty((q.shape[0], q.shape[2], q.shape[1], q.shape[3]))
+
+    if hasattr(torch.ops.xinfer, "paged_attention_kv4"):
+        from xinfer_amd.paged_kv4 import register_fakes
+
+        register_fakes()
 
     _loaded = library
 

@@ -28,9 +28,9 @@ LIBRARY_NAME = "libxinfer_attention_ops.so"
 ARCH = "gfx950"
 
 KERNEL_SOURCES = ("append.hip", "decode.hip", "prefill.hip", "prefill_d256.hip", "merge.hip", "norm_rope.hip",
-                  "gemv.hip", "scratch.hip")
-HOST_SOURCES = ("capi.cpp",)
-TORCH_SOURCES = ("torch_ops.cpp",)
+                  "gemv.hip", "scratch.hip", "kv4_cache.hip", "paged_reserve.hip", "paged_attention.hip")
+HOST_SOURCES = ("capi.cpp", "kv4_capi.cpp")
+TORCH_SOURCES = ("torch_ops.cpp", "kv4_ops.cpp")
 
 # Packed fp32 VALU instructions are kept out of every device build.
 NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]

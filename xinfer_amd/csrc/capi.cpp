@@ -1024,6 +1024,12 @@ const char *xinfer_status_string(int status) {
       return "Graph-capture attention takes at most 64 rows";
     case XINFER_ERR_SCRATCH:
       return "Attention needs more split-record scratch than the allocation-free entry point holds (32 MiB)";
+    case XINFER_ERR_KV4_CACHE:
+      return "Expected a 4-bit KV cache with head dim in {64,128,256}, pages of 64, 128 or 256 tokens and 16-byte "
+             "aligned data";
+    case XINFER_ERR_KV4_SHAPE: return "Tensors do not match the 4-bit KV cache or each other";
+    case XINFER_ERR_PAGES:
+      return "Expected pages of 64, 128 or 256 tokens, and a page table and a ring of free pages below 2^31 entries";
     default: return "Unknown xinfer status";
   }
 }

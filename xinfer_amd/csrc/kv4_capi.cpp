@@ -1,0 +1,199 @@
+// C ABI of the paged 4-bit KV cache (include/xinfer_attention.h): validation and launches.
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+#include <limits>
+
+#include "xinfer_attention.h"
+#include "kv4_common.h"
+#include "launch.h"
+
+namespace xattn {
+namespace {
+
+constexpr int64_t kIntMax = std::numeric_limits<int32_t>::max();
+
+bool aligned16(const void *p) { return p != nullptr && (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+int page_shift(int64_t page_size) { return page_size == 64 ? 6 : page_size == 128 ? 7 : page_size == 256 ? 8 : -1; }
+
+bool cache_of(const xinfer_kv4_cache &c, Kv4Cache &out) {
+  if (page_shift(c.page_size) < 0 || (c.dim != 64 && c.dim != 128 && c.dim != 256)) return false;
+  // Pages are counted in 32 bits (a table's entries); places inside the cache are 64-bit.
+  if (c.pages < 1 || c.pages > kIntMax || c.kv_heads < 1 || c.kv_heads > 65535) return false;
+  for (const void *p : {c.key, c.key_scale, c.value, c.value_scale})
+    if (!aligned16(p)) return false;
+  out = Kv4Cache{static_cast<uint8_t *>(c.key), static_cast<uint8_t *>(c.key_scale), static_cast<uint8_t *>(c.value),
+                 static_cast<uint8_t *>(c.value_scale), c.pages, (int32_t)c.kv_heads, (int32_t)c.dim,
+                 page_shift(c.page_size)};
+  return true;
+}
+
+// 16-byte rows: unit feature stride, other strides divisible by 8, aligned data.
+bool rows_ok(const xinfer_view4 &t) {
+  if (!aligned16(t.data) || (t.size[3] > 1 && t.stride[3] != 1)) return false;
+  for (int i = 0; i < 3; ++i)
+    if (t.size[i] > 1 && t.stride[i] % 8 != 0) return false;
+  return true;
+}
+
+// key/value [B, Hkv, T, D] of the cache; B * T * heads rows are counted in 32 bits.
+bool new_tokens_ok(const xinfer_view4 &key, const xinfer_view4 &value, const Kv4Cache &cache, int64_t heads) {
+  for (int i = 0; i < 4; ++i)
+    if (key.size[i] < 0 || value.size[i] != key.size[i]) return false;
+  return key.size[1] == cache.Hkv && key.size[3] == cache.D && key.size[0] <= kIntMax && key.size[2] <= kIntMax &&
+         (key.size[0] == 0 || key.size[2] <= kIntMax / key.size[0]) &&
+         key.size[0] * key.size[2] <= (kIntMax - 1024) / heads;
+}
+
+View view_of(const xinfer_view4 &t) {
+  return View{static_cast<const uint16_t *>(t.data), t.stride[0], t.stride[1], t.stride[2]};
+}
+
+int done(hipError_t e) { return e == hipSuccess ? XINFER_OK : XINFER_ERR_LAUNCH; }
+
+}  // namespace
+}  // namespace xattn
+
+using namespace xattn;
+
+extern "C" {
+
+int xinfer_paged_kv_reserve(const int32_t *kv_before, const int32_t *kv_lengths, const int32_t *query_lengths,
+                            int64_t rows, int64_t tokens, int64_t page_size, const int64_t *counters,
+                            int32_t *block_table, int64_t table_width, int32_t *free_pages, int64_t ring_size,
+                            int32_t *lengths, int64_t *positions, int64_t *slots, int64_t *new_counters,
+                            void *stream) {
+  const int shift = page_shift(page_size);
+  if (shift < 0 || table_width < 1 || table_width > kIntMax >> shift || ring_size < 1 || ring_size > kIntMax)
+    return XINFER_ERR_PAGES;
+  if (rows < 0 || tokens < 0 || tokens > kIntMax) return XINFER_ERR_ARGUMENT;
+  if (rows > kIntMax / table_width) return XINFER_ERR_PAGES;
+  if (!counters || !new_counters || counters == new_counters) return XINFER_ERR_ARGUMENT;
+  if (rows > 0 && (!kv_before || !kv_lengths || !query_lengths || !block_table || !free_pages || !lengths))
+    return XINFER_ERR_ARGUMENT;
+  if (rows > 0 && tokens > 0 && (!positions || !slots)) return XINFER_ERR_ARGUMENT;
+  const ReserveArgs a{kv_before, kv_lengths, query_lengths, counters, block_table, free_pages, lengths, positions, slots,
+                      new_counters, ring_size, (int32_t)rows, (int32_t)tokens, (int32_t)table_width, shift};
+  return done(launch_reserve(a, static_cast<hipStream_t>(stream)));
+}
+
+int xinfer_append_kv4(const xinfer_view4 *key, const xinfer_view4 *value, const int64_t *slots,
+                      int64_t slot_stride_b, int64_t slot_stride_t, const xinfer_kv4_cache *cache, void *stream) {
+  if (!key || !value || !cache) return XINFER_ERR_ARGUMENT;
+  Kv4AppendArgs a{};
+  if (!cache_of(*cache, a.cache)) return XINFER_ERR_KV4_CACHE;
+  if (!new_tokens_ok(*key, *value, a.cache, a.cache.Hkv)) return XINFER_ERR_KV4_SHAPE;
+  if (key->size[0] == 0 || key->size[2] == 0) return XINFER_OK;
+  if (!slots) return XINFER_ERR_ARGUMENT;
+  if (!rows_ok(*key) || !rows_ok(*value)) return XINFER_ERR_LAYOUT;
+  a.key = view_of(*key);
+  a.value = view_of(*value);
+  a.slots = slots;
+  a.slot_sb = slot_stride_b;
+  a.slot_st = slot_stride_t;
+  a.B = (int32_t)key->size[0];
+  a.T = (int32_t)key->size[2];
+  return done(launch_append_kv4(a, static_cast<hipStream_t>(stream)));
+}
+
+int xinfer_read_kv4(const xinfer_kv4_cache *cache, const int64_t *slots, int64_t slot_stride_b,
+                    int64_t slot_stride_t, int64_t batch, int64_t tokens, void *key, void *value, void *stream) {
+  if (!cache) return XINFER_ERR_ARGUMENT;
+  Kv4ReadArgs a{};
+  if (!cache_of(*cache, a.cache)) return XINFER_ERR_KV4_CACHE;
+  const xinfer_view4 out{key, {batch, cache->kv_heads, tokens, cache->dim}, {0, 0, 0, 1}};
+  if (!new_tokens_ok(out, out, a.cache, a.cache.Hkv)) return XINFER_ERR_KV4_SHAPE;
+  if (batch == 0 || tokens == 0) return XINFER_OK;
+  if (!slots) return XINFER_ERR_ARGUMENT;
+  if (!aligned16(key) || !aligned16(value)) return XINFER_ERR_LAYOUT;
+  a.slots = slots;
+  a.slot_sb = slot_stride_b;
+  a.slot_st = slot_stride_t;
+  a.key = static_cast<uint16_t *>(key);
+  a.value = static_cast<uint16_t *>(value);
+  a.B = (int32_t)batch;
+  a.T = (int32_t)tokens;
+  return done(launch_read_kv4(a, static_cast<hipStream_t>(stream)));
+}
+
+int xinfer_qk_norm_rope_append_kv4(const xinfer_view4 *q, const xinfer_view4 *key, const xinfer_view4 *value,
+                                   const void *q_weight, const void *k_weight, double eps, double weight_offset,
+                                   const xinfer_view4 *cos, const xinfer_view4 *sin, const int64_t *slots,
+                                   int64_t slot_stride_b, int64_t slot_stride_t, void *q_out,
+                                   const xinfer_kv4_cache *cache, void *stream) {
+  if (!q || !key || !value || !cos || !sin || !cache) return XINFER_ERR_ARGUMENT;
+  Kv4NormRopeArgs a{};
+  if (!cache_of(*cache, a.cache)) return XINFER_ERR_KV4_CACHE;
+  const int64_t B = key->size[0], T = key->size[2], Hq = q->size[1], R = cos->size[3];
+  if (q->size[0] != B || q->size[2] != T || q->size[3] != a.cache.D || Hq < 1 || Hq > 65535 ||
+      !new_tokens_ok(*key, *value, a.cache, Hq + a.cache.Hkv) || R < 16 || R > a.cache.D || R % 16 != 0)
+    return XINFER_ERR_KV4_SHAPE;
+  for (const xinfer_view4 *r : {cos, sin})
+    if (r->size[0] != B || r->size[1] != 1 || r->size[2] != T || r->size[3] != R) return XINFER_ERR_KV4_SHAPE;
+  if (!(std::isfinite(eps) && eps >= 0)) return XINFER_ERR_EPS;
+  if (!std::isfinite(weight_offset)) return XINFER_ERR_ARGUMENT;
+  if (B == 0 || T == 0) return XINFER_OK;
+  if (!q_weight || !k_weight || !slots || !q_out) return XINFER_ERR_ARGUMENT;
+  for (const xinfer_view4 *t : {q, key, value, cos, sin})
+    if (!rows_ok(*t)) return XINFER_ERR_LAYOUT;
+  for (const void *p : {q_weight, k_weight, static_cast<const void *>(q_out)})
+    if (!aligned16(p)) return XINFER_ERR_LAYOUT;
+  a.q = view_of(*q);
+  a.k = view_of(*key);
+  a.v = view_of(*value);
+  a.q_weight = static_cast<const uint16_t *>(q_weight);
+  a.k_weight = static_cast<const uint16_t *>(k_weight);
+  a.cos = view_of(*cos);
+  a.sin = view_of(*sin);
+  a.slots = slots;
+  a.slot_sb = slot_stride_b;
+  a.slot_st = slot_stride_t;
+  a.q_out = static_cast<uint16_t *>(q_out);
+  a.eps = (float)eps;
+  a.offset = (float)weight_offset;
+  a.B = (int32_t)B;
+  a.T = (int32_t)T;
+  a.Hq = (int32_t)Hq;
+  a.R = (int32_t)R;
+  return done(launch_norm_rope_kv4(a, static_cast<hipStream_t>(stream)));
+}
+
+size_t xinfer_paged_attention_kv4_workspace_size(const xinfer_view4 *q, const xinfer_kv4_cache *cache,
+                                                 int64_t table_width, int64_t max_length) {
+  (void)q, (void)cache, (void)table_width, (void)max_length;
+  return 0;
+}
+
+int xinfer_paged_attention_kv4(const xinfer_view4 *q, const xinfer_kv4_cache *cache, const int32_t *block_table,
+                               int64_t table_width, const int32_t *lengths, int64_t max_length, double scale,
+                               void *out, void *workspace, size_t workspace_bytes, void *stream) {
+  if (!q || !cache) return XINFER_ERR_ARGUMENT;
+  PagedArgs a{};
+  if (!cache_of(*cache, a.cache)) return XINFER_ERR_KV4_CACHE;
+  const int64_t B = q->size[0], Hq = q->size[1], T = q->size[2];
+  if (B < 0 || B > 65535 || T < 0 || q->size[3] != a.cache.D) return XINFER_ERR_KV4_SHAPE;
+  if (Hq < 1 || Hq > 65535 || Hq % a.cache.Hkv != 0) return XINFER_ERR_HEADS;
+  if (table_width < 1 || table_width > kIntMax >> a.cache.page_shift || max_length < 0) return XINFER_ERR_PAGES;
+  if (T > (kIntMax >> 8) / Hq || B * Hq * T > kIntMax >> 4) return XINFER_ERR_KV4_SHAPE;
+  if (!(std::isfinite(scale) && scale > 0)) return XINFER_ERR_SCALE;
+  if (B == 0 || T == 0) return XINFER_OK;
+  if (!block_table || !lengths || !out) return XINFER_ERR_ARGUMENT;
+  if (!rows_ok(*q) || !aligned16(out)) return XINFER_ERR_LAYOUT;
+  (void)workspace, (void)workspace_bytes;
+  const int64_t capacity = table_width << a.cache.page_shift;
+  a.q = view_of(*q);
+  a.table = block_table;
+  a.lengths = lengths;
+  a.out = static_cast<uint16_t *>(out);
+  a.scale_log2 = (float)(scale * 1.4426950408889634);
+  a.B = (int32_t)B;
+  a.Hq = (int32_t)Hq;
+  a.G = (int32_t)(Hq / a.cache.Hkv);
+  a.T = (int32_t)T;
+  a.width = (int32_t)table_width;
+  a.max_length = (int32_t)(max_length == 0 ? capacity : std::min(max_length, capacity));
+  return done(launch_paged_attention(a, static_cast<hipStream_t>(stream)));
+}
+
+}  // extern "C"

@@ -1,0 +1,218 @@
+// torch.library registration and AOTInductor C shims of the paged 4-bit KV cache: a thin layer over the C ABI
+// (include/xinfer_attention.h), as torch_ops.cpp is over the other operators.  Outputs and workspaces come from the
+// caching allocator, launches go to the current stream of the inputs' device.
+#include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
+#include <torch/csrc/inductor/aoti_torch/utils.h>
+#include <torch/library.h>
+
+#include <cmath>
+#include <initializer_list>
+#include <tuple>
+
+#include "xinfer_attention.h"
+#include "xinfer_attention_aoti.h"
+
+namespace xinfer {
+namespace {
+
+using Tensors = std::initializer_list<const at::Tensor *>;
+
+xinfer_view4 view4(const at::Tensor &t) {
+  xinfer_view4 v{};
+  v.data = t.data_ptr();
+  for (int i = 0; i < 4; ++i) {
+    v.size[i] = t.size(i);
+    v.stride[i] = t.stride(i);
+  }
+  return v;
+}
+
+// Rows the kernels read in place: unit feature stride, other strides divisible by 8, 16-byte aligned data; others
+// are copied.
+at::Tensor in_rows(const at::Tensor &t) {
+  bool fine = (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) == 0 && (t.size(3) <= 1 || t.stride(3) == 1);
+  for (int i = 0; i < 3; ++i) fine = fine && (t.size(i) <= 1 || t.stride(i) % 8 == 0);
+  return fine ? t : t.contiguous(at::MemoryFormat::Contiguous);
+}
+
+void *stream_of(const at::Tensor &t) {
+  return static_cast<void *>(c10::hip::getCurrentHIPStream(t.device().index()).stream());
+}
+
+void check_status(int status) { TORCH_CHECK(status == XINFER_OK, xinfer_status_string(status)); }
+
+void check_colocated(const at::Tensor &first, Tensors others) {
+  bool fine = first.is_cuda();
+  for (const at::Tensor *t : others) fine = fine && t->device() == first.device();
+  TORCH_CHECK(fine, "xinfer paged KV cache requires colocated CUDA tensors");
+}
+
+void check_bf16(Tensors tensors) {
+  for (const at::Tensor *t : tensors)
+    TORCH_CHECK(t->scalar_type() == at::kBFloat16, "xinfer paged KV cache requires BF16 activations and weights");
+}
+
+xinfer_kv4_cache cache_of(const at::Tensor &key, const at::Tensor &key_scale, const at::Tensor &value,
+                          const at::Tensor &value_scale) {
+  bool fine = true;
+  for (const at::Tensor *t : {&key, &key_scale, &value, &value_scale})
+    fine = fine && t->scalar_type() == at::kByte && t->dim() == 4 && t->is_contiguous() && t->device() == key.device();
+  TORCH_CHECK(fine, "Expected contiguous uint8 cache tensors of four dimensions on one device");
+  TORCH_CHECK(value.sizes() == key.sizes() && value_scale.sizes() == key_scale.sizes() &&
+                  key_scale.size(0) == key.size(0) && key_scale.size(1) == key.size(1) &&
+                  key_scale.size(3) == key.size(2) && key_scale.size(2) * 16 == key.size(3),
+              "Expected cache codes [N,Hkv,P,D/2] and scales [N,Hkv,D/32,P]");
+  return xinfer_kv4_cache{key.data_ptr(),  key_scale.data_ptr(), value.data_ptr(), value_scale.data_ptr(),
+                          key.size(0),     key.size(1),          key.size(2),      2 * key.size(3)};
+}
+
+void check_slots(const at::Tensor &slots, int64_t batch, int64_t tokens) {
+  TORCH_CHECK(slots.scalar_type() == at::kLong && slots.dim() == 2 && slots.size(0) == batch && slots.size(1) == tokens,
+              "Expected int64 slots [B,T]");
+}
+
+}  // namespace
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> paged_kv_reserve(
+    const at::Tensor &kv_before, const at::Tensor &kv_lengths, const at::Tensor &query_lengths, int64_t tokens,
+    int64_t page_size, const at::Tensor &counters, const at::Tensor &block_table, const at::Tensor &free_pages) {
+  check_colocated(kv_before, {&kv_lengths, &query_lengths, &counters, &block_table, &free_pages});
+  TORCH_CHECK(kv_before.dim() == 1, "Expected int32 row lengths [B]");
+  const int64_t rows = kv_before.size(0);
+  for (const at::Tensor *t : {&kv_before, &kv_lengths, &query_lengths})
+    TORCH_CHECK(t->scalar_type() == at::kInt && t->dim() == 1 && t->size(0) == rows, "Expected int32 row lengths [B]");
+  TORCH_CHECK(counters.scalar_type() == at::kLong && counters.dim() == 1 && counters.size(0) == 2 &&
+                  counters.is_contiguous(),
+              "Expected int64 counters [2]");
+  TORCH_CHECK(block_table.scalar_type() == at::kInt && block_table.dim() == 2 && block_table.size(0) == rows &&
+                  block_table.is_contiguous(),
+              "Expected a contiguous int32 block table [B,M]");
+  TORCH_CHECK(free_pages.scalar_type() == at::kInt && free_pages.dim() == 1 && free_pages.is_contiguous(),
+              "Expected a contiguous int32 ring of free pages");
+  TORCH_CHECK(tokens >= 0, "Expected a number of new tokens");
+  c10::DeviceGuard guard(kv_before.device());
+  auto before = kv_before.contiguous(), after = kv_lengths.contiguous(), counts = query_lengths.contiguous();
+  auto lengths = at::empty({2, rows}, kv_before.options());
+  auto positions = at::empty({rows, tokens}, counters.options()), slots = at::empty({rows, tokens}, counters.options());
+  auto next = at::empty({2}, counters.options());
+  auto ints = [](const at::Tensor &t) { return static_cast<int32_t *>(t.data_ptr()); };
+  auto longs = [](const at::Tensor &t) { return static_cast<int64_t *>(t.data_ptr()); };
+  check_status(xinfer_paged_kv_reserve(ints(before), ints(after), ints(counts), rows, tokens, page_size, longs(counters),
+                                       ints(block_table), block_table.size(1), ints(free_pages), free_pages.size(0),
+                                       ints(lengths), longs(positions), longs(slots), longs(next),
+                                       stream_of(kv_before)));
+  return {lengths, positions, slots, next};
+}
+
+void append_kv4(const at::Tensor &key, const at::Tensor &value, const at::Tensor &slots, const at::Tensor &key_codes,
+                const at::Tensor &key_scales, const at::Tensor &value_codes, const at::Tensor &value_scales) {
+  check_colocated(key, {&value, &slots, &key_codes, &key_scales, &value_codes, &value_scales});
+  TORCH_CHECK(key.dim() == 4 && value.sizes() == key.sizes(), "Expected key/value [B,Hkv,T,D]");
+  check_bf16({&key, &value});
+  check_slots(slots, key.size(0), key.size(2));
+  const auto cache = cache_of(key_codes, key_scales, value_codes, value_scales);
+  c10::DeviceGuard guard(key.device());
+  auto k = in_rows(key), v = in_rows(value);
+  auto kv = view4(k), vv = view4(v);
+  check_status(xinfer_append_kv4(&kv, &vv, static_cast<const int64_t *>(slots.data_ptr()), slots.stride(0),
+                                 slots.stride(1), &cache, stream_of(key)));
+}
+
+std::tuple<at::Tensor, at::Tensor> read_kv4(const at::Tensor &key_codes, const at::Tensor &key_scales,
+                                            const at::Tensor &value_codes, const at::Tensor &value_scales,
+                                            const at::Tensor &slots) {
+  check_colocated(key_codes, {&key_scales, &value_codes, &value_scales, &slots});
+  TORCH_CHECK(slots.scalar_type() == at::kLong && slots.dim() == 2, "Expected int64 slots [B,T]");
+  const auto cache = cache_of(key_codes, key_scales, value_codes, value_scales);
+  c10::DeviceGuard guard(slots.device());
+  const auto options = slots.options().dtype(at::kBFloat16);
+  auto key = at::empty({slots.size(0), cache.kv_heads, slots.size(1), cache.dim}, options);
+  auto value = at::empty(key.sizes(), options);
+  check_status(xinfer_read_kv4(&cache, static_cast<const int64_t *>(slots.data_ptr()), slots.stride(0), slots.stride(1),
+                               slots.size(0), slots.size(1), key.data_ptr(), value.data_ptr(), stream_of(slots)));
+  return {key, value};
+}
+
+at::Tensor qk_norm_rope_append_kv4(const at::Tensor &q, const at::Tensor &key, const at::Tensor &value,
+                                   const at::Tensor &q_weight, const at::Tensor &k_weight, double eps,
+                                   double weight_offset, const at::Tensor &cos, const at::Tensor &sin,
+                                   const at::Tensor &slots, const at::Tensor &key_codes, const at::Tensor &key_scales,
+                                   const at::Tensor &value_codes, const at::Tensor &value_scales) {
+  check_colocated(q, {&key, &value, &q_weight, &k_weight, &cos, &sin, &slots, &key_codes, &key_scales, &value_codes,
+                      &value_scales});
+  TORCH_CHECK(q.dim() == 4 && key.dim() == 4 && value.sizes() == key.sizes() && key.size(0) == q.size(0) &&
+                  key.size(1) == q.size(1) && key.size(3) == q.size(3) && cos.dim() == 3 && cos.sizes() == sin.sizes() &&
+                  cos.size(0) == q.size(0) && cos.size(1) == q.size(1) && q_weight.dim() == 1 &&
+                  q_weight.size(0) == q.size(3) && k_weight.sizes() == q_weight.sizes(),
+              "Expected q [B,T,Hq,D], key/value [B,T,Hkv,D], cos/sin [B,T,R] and [D] weights");
+  check_bf16({&q, &key, &value, &q_weight, &k_weight, &cos, &sin});
+  check_slots(slots, q.size(0), q.size(1));
+  const auto cache = cache_of(key_codes, key_scales, value_codes, value_scales);
+  c10::DeviceGuard guard(q.device());
+  auto output = at::empty({q.size(0), q.size(2), q.size(1), q.size(3)}, q.options());
+  // Per-head views [B,H,T,D] and [B,1,T,R].
+  auto qh = in_rows(q.transpose(1, 2)), kh = in_rows(key.transpose(1, 2)), vh = in_rows(value.transpose(1, 2));
+  auto cs = in_rows(cos.unsqueeze(1)), sn = in_rows(sin.unsqueeze(1));
+  // in_rows of a rank-4 view: the weights as one row.
+  auto qw = in_rows(q_weight.view({1, 1, 1, -1})), kw = in_rows(k_weight.view({1, 1, 1, -1}));
+  auto qv = view4(qh), kv = view4(kh), vv = view4(vh), cv = view4(cs), sv = view4(sn);
+  check_status(xinfer_qk_norm_rope_append_kv4(&qv, &kv, &vv, qw.data_ptr(), kw.data_ptr(), eps, weight_offset, &cv, &sv,
+                                              static_cast<const int64_t *>(slots.data_ptr()), slots.stride(0),
+                                              slots.stride(1), output.data_ptr(), &cache, stream_of(q)));
+  return output;
+}
+
+at::Tensor paged_attention_kv4(const at::Tensor &q, const at::Tensor &key_codes, const at::Tensor &key_scales,
+                               const at::Tensor &value_codes, const at::Tensor &value_scales,
+                               const at::Tensor &block_table, const at::Tensor &lengths, int64_t max_length,
+                               double scale) {
+  check_colocated(q, {&key_codes, &key_scales, &value_codes, &value_scales, &block_table, &lengths});
+  TORCH_CHECK(q.dim() == 4, "Expected q [B,Hq,T,D]");
+  check_bf16({&q});
+  TORCH_CHECK(block_table.scalar_type() == at::kInt && block_table.dim() == 2 && block_table.size(0) == q.size(0) &&
+                  block_table.is_contiguous(),
+              "Expected a contiguous int32 block table [B,M]");
+  TORCH_CHECK(lengths.scalar_type() == at::kInt && lengths.dim() == 2 && lengths.size(0) == 2 &&
+                  lengths.size(1) == q.size(0) && lengths.is_contiguous(),
+              "Expected contiguous int32 lengths [2,B]");
+  TORCH_CHECK(!q.requires_grad(), "xinfer attention supports inference only");
+  const auto cache = cache_of(key_codes, key_scales, value_codes, value_scales);
+  c10::DeviceGuard guard(q.device());
+  auto output = at::empty({q.size(0), q.size(2), q.size(1), q.size(3)}, q.options());
+  auto query = in_rows(q);
+  auto qv = view4(query);
+  const size_t bytes = xinfer_paged_attention_kv4_workspace_size(&qv, &cache, block_table.size(1), max_length);
+  auto workspace = at::empty({static_cast<int64_t>(bytes)}, q.options().dtype(at::kByte));
+  check_status(xinfer_paged_attention_kv4(&qv, &cache, static_cast<const int32_t *>(block_table.data_ptr()),
+                                          block_table.size(1), static_cast<const int32_t *>(lengths.data_ptr()),
+                                          max_length, scale, output.data_ptr(), workspace.data_ptr(), bytes,
+                                          stream_of(q)));
+  return output;
+}
+
+}  // namespace xinfer
+
+TORCH_LIBRARY_FRAGMENT(xinfer, m) {
+  m.def("paged_kv_reserve(Tensor kv_before, Tensor kv_lengths, Tensor query_lengths, SymInt tokens, SymInt page_size, "
+        "Tensor counters, Tensor(a6!) block_table, Tensor(a7!) free_pages) -> (Tensor, Tensor, Tensor, Tensor)");
+  m.def("append_kv4(Tensor key, Tensor value, Tensor slots, Tensor(a3!) key_codes, Tensor(a4!) key_scales, "
+        "Tensor(a5!) value_codes, Tensor(a6!) value_scales) -> ()");
+  m.def("read_kv4(Tensor key_codes, Tensor key_scales, Tensor value_codes, Tensor value_scales, Tensor slots) "
+        "-> (Tensor, Tensor)");
+  m.def("qk_norm_rope_append_kv4(Tensor q, Tensor key, Tensor value, Tensor q_weight, Tensor k_weight, float eps, "
+        "float weight_offset, Tensor cos, Tensor sin, Tensor slots, Tensor(a10!) key_codes, Tensor(a11!) key_scales, "
+        "Tensor(a12!) value_codes, Tensor(a13!) value_scales) -> Tensor");
+  m.def("paged_attention_kv4(Tensor q, Tensor key_codes, Tensor key_scales, Tensor value_codes, Tensor value_scales, "
+        "Tensor block_table, Tensor lengths, SymInt max_length, float scale) -> Tensor",
+        {at::Tag::flexible_layout});
+}
+
+TORCH_LIBRARY_IMPL(xinfer, CUDA, m) {
+  m.impl("paged_kv_reserve", TORCH_FN(xinfer::paged_kv_reserve));
+  m.impl("append_kv4", TORCH_FN(xinfer::append_kv4));
+  m.impl("read_kv4", TORCH_FN(xinfer::read_kv4));
+  m.impl("qk_norm_rope_append_kv4", TORCH_FN(xinfer::qk_norm_rope_append_kv4));
+  m.impl("paged_attention_kv4", TORCH_FN(xinfer::paged_attention_kv4));
+}

@@ -4,6 +4,7 @@
 #include <hip/hip_runtime_api.h>
 
 #include "kernel_args.h"
+#include "kv4_common.h"
 
 namespace xattn {
 
@@ -73,5 +74,12 @@ constexpr size_t kScratchBytes = size_t(32) << 20;
 // The current device's address of that scratch (scratch.hip), looked up once
 // per device.
 hipError_t scratch_pointer(void **pointer);
+
+// The paged 4-bit KV cache (kv4_cache.hip, paged_reserve.hip, paged_attention.hip).
+hipError_t launch_append_kv4(const Kv4AppendArgs &a, hipStream_t stream);
+hipError_t launch_read_kv4(const Kv4ReadArgs &a, hipStream_t stream);
+hipError_t launch_norm_rope_kv4(const Kv4NormRopeArgs &a, hipStream_t stream);
+hipError_t launch_reserve(const ReserveArgs &a, hipStream_t stream);
+hipError_t launch_paged_attention(const PagedArgs &a, hipStream_t stream);
 
 }  // namespace xattn
