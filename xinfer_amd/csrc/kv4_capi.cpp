@@ -50,6 +50,65 @@ View view_of(const xinfer_view4 &t) {
   return View{static_cast<const uint16_t *>(t.data), t.stride[0], t.stride[1], t.stride[2]};
 }
 
+// Launches and workspace of a paged attention call, from the shapes and the bound on the lengths alone.  Rows of few
+// query vectors go to the decode kernel, the others, where the shapes allow any, to the prefill kernel.
+struct PagedLaunch {
+  PagedArgs a;
+  int64_t items;
+  int tiles;     // of a row and KV head, at most
+  size_t bytes;  // records of rows cut into runs; 0: no row can be
+};
+constexpr int kPagedTarget = 512;  // items that fill the chip: two blocks a CU
+constexpr int kPagedDecodeGroups = 16, kPagedPrefillGroups = 8;
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+PagedLaunch paged_launch(const PagedArgs &shapes, int vectors_min, int vectors_max, int tile, int min_groups) {
+  PagedLaunch l{shapes, 0, 0, 0};
+  l.a.vectors_min = vectors_min;
+  l.a.vectors_max = vectors_max;
+  l.a.tile = tile;
+  l.a.min_groups = min_groups;
+  l.a.target = kPagedTarget;
+  l.tiles = (int)ceil_div(std::min<int64_t>((int64_t)shapes.T * shapes.G, vectors_max), tile);
+  // A row and tile has at most one run more than its share of the target.
+  const int64_t whole = (int64_t)shapes.B * shapes.cache.Hkv * l.tiles;
+  const int64_t runs = ceil_div(ceil_div(shapes.max_length, 64), min_groups);
+  l.items = runs <= 1 ? whole : std::min(whole * runs, whole + kPagedTarget);
+  l.bytes = runs <= 1 ? 0 : (size_t)l.items * tile * (shapes.cache.D + 2) * sizeof(float);
+  return l;
+}
+
+struct PagedCall {
+  PagedLaunch few, many;
+  bool both;
+  size_t bytes() const { return few.bytes + (both ? many.bytes : 0); }
+};
+
+int paged_call(const xinfer_view4 &q, const xinfer_kv4_cache &cache, int64_t table_width, int64_t max_length,
+               PagedCall &call) {
+  PagedArgs a{};
+  if (!cache_of(cache, a.cache)) return XINFER_ERR_KV4_CACHE;
+  const int64_t B = q.size[0], Hq = q.size[1], T = q.size[2];
+  if (B < 0 || B > 65535 || T < 0 || q.size[3] != a.cache.D) return XINFER_ERR_KV4_SHAPE;
+  if (Hq < 1 || Hq > 65535 || Hq % a.cache.Hkv != 0) return XINFER_ERR_HEADS;
+  if (table_width < 1 || table_width > kIntMax >> a.cache.page_shift || max_length < 0) return XINFER_ERR_PAGES;
+  // Query vectors and items are counted in 32 bits.
+  if (T > (kIntMax >> 8) / Hq || B * Hq * T > kIntMax >> 4) return XINFER_ERR_KV4_SHAPE;
+  const int64_t capacity = table_width << a.cache.page_shift;
+  a.B = (int32_t)B;
+  a.Hq = (int32_t)Hq;
+  a.G = (int32_t)(Hq / a.cache.Hkv);
+  a.T = (int32_t)T;
+  a.width = (int32_t)table_width;
+  a.max_length = (int32_t)(max_length == 0 ? capacity : std::min(max_length, capacity));
+  const int columns = paged_decode_columns(a.cache.D), vectors = a.T * a.G;
+  call.few = paged_launch(a, 0, vectors <= 32 ? 32 : columns, vectors <= 16 ? 16 : columns, kPagedDecodeGroups);
+  call.both = vectors > 32;
+  if (call.both) call.many = paged_launch(a, columns + 1, kIntMax, kPagedPrefillTile, kPagedPrefillGroups);
+  return XINFER_OK;
+}
+
 int done(hipError_t e) { return e == hipSuccess ? XINFER_OK : XINFER_ERR_LAUNCH; }
 
 }  // namespace
@@ -161,39 +220,41 @@ int xinfer_qk_norm_rope_append_kv4(const xinfer_view4 *q, const xinfer_view4 *ke
 
 size_t xinfer_paged_attention_kv4_workspace_size(const xinfer_view4 *q, const xinfer_kv4_cache *cache,
                                                  int64_t table_width, int64_t max_length) {
-  (void)q, (void)cache, (void)table_width, (void)max_length;
-  return 0;
+  PagedCall call{};
+  if (!q || !cache || paged_call(*q, *cache, table_width, max_length, call) != XINFER_OK) return 0;
+  return call.bytes();
 }
 
 int xinfer_paged_attention_kv4(const xinfer_view4 *q, const xinfer_kv4_cache *cache, const int32_t *block_table,
                                int64_t table_width, const int32_t *lengths, int64_t max_length, double scale,
                                void *out, void *workspace, size_t workspace_bytes, void *stream) {
   if (!q || !cache) return XINFER_ERR_ARGUMENT;
-  PagedArgs a{};
-  if (!cache_of(*cache, a.cache)) return XINFER_ERR_KV4_CACHE;
-  const int64_t B = q->size[0], Hq = q->size[1], T = q->size[2];
-  if (B < 0 || B > 65535 || T < 0 || q->size[3] != a.cache.D) return XINFER_ERR_KV4_SHAPE;
-  if (Hq < 1 || Hq > 65535 || Hq % a.cache.Hkv != 0) return XINFER_ERR_HEADS;
-  if (table_width < 1 || table_width > kIntMax >> a.cache.page_shift || max_length < 0) return XINFER_ERR_PAGES;
-  if (T > (kIntMax >> 8) / Hq || B * Hq * T > kIntMax >> 4) return XINFER_ERR_KV4_SHAPE;
+  PagedCall call{};
+  const int status = paged_call(*q, *cache, table_width, max_length, call);
+  if (status != XINFER_OK) return status;
   if (!(std::isfinite(scale) && scale > 0)) return XINFER_ERR_SCALE;
-  if (B == 0 || T == 0) return XINFER_OK;
+  if (q->size[0] == 0 || q->size[2] == 0) return XINFER_OK;
   if (!block_table || !lengths || !out) return XINFER_ERR_ARGUMENT;
   if (!rows_ok(*q) || !aligned16(out)) return XINFER_ERR_LAYOUT;
-  (void)workspace, (void)workspace_bytes;
-  const int64_t capacity = table_width << a.cache.page_shift;
-  a.q = view_of(*q);
-  a.table = block_table;
-  a.lengths = lengths;
-  a.out = static_cast<uint16_t *>(out);
-  a.scale_log2 = (float)(scale * 1.4426950408889634);
-  a.B = (int32_t)B;
-  a.Hq = (int32_t)Hq;
-  a.G = (int32_t)(Hq / a.cache.Hkv);
-  a.T = (int32_t)T;
-  a.width = (int32_t)table_width;
-  a.max_length = (int32_t)(max_length == 0 ? capacity : std::min(max_length, capacity));
-  return done(launch_paged_attention(a, static_cast<hipStream_t>(stream)));
+  if (call.bytes() > 0 && (!aligned16(workspace) || workspace_bytes < call.bytes())) return XINFER_ERR_WORKSPACE;
+  uint8_t *records = static_cast<uint8_t *>(workspace);
+  for (PagedLaunch *l : {&call.few, &call.many}) {
+    l->a.q = view_of(*q);
+    l->a.table = block_table;
+    l->a.lengths = lengths;
+    l->a.out = static_cast<uint16_t *>(out);
+    l->a.scale_log2 = (float)(scale * 1.4426950408889634);
+    l->a.part_o = reinterpret_cast<float *>(records);
+    l->a.part_ml = l->a.part_o + l->items * l->a.tile * l->a.cache.D;
+    records += l->bytes;
+  }
+  const hipStream_t on = static_cast<hipStream_t>(stream);
+  if (call.both && launch_paged_prefill(call.many.a, (unsigned)call.many.items, on) != hipSuccess)
+    return XINFER_ERR_LAUNCH;
+  if (launch_paged_decode(call.few.a, (unsigned)call.few.items, on) != hipSuccess) return XINFER_ERR_LAUNCH;
+  if (call.bytes() == 0) return XINFER_OK;
+  return done(launch_paged_merge(call.few.a, call.both ? &call.many.a : nullptr,
+                                 std::max(call.few.tiles, call.both ? call.many.tiles : 0), on));
 }
 
 }  // extern "C"

@@ -1,4 +1,5 @@
-// The 4-bit KV cache's format and arguments (kv4_cache.hip, paged_reserve.hip, paged_attention.hip).
+// The 4-bit KV cache's format and arguments (kv4_cache.hip, paged_reserve.hip, paged_decode.hip,
+// paged_prefill.hip).
 //
 // A key or value vector is held as blocks of 32 features: codes e2m1 (a sign and a magnitude of 0, 0.5, 1, 1.5, 2,
 // 3, 4 or 6, the even feature in a byte's low half) and an e8m0 scale byte s for 2^(s - 127), the operand format of
@@ -79,6 +80,12 @@ struct PagedArgs {
   float scale_log2;
   int32_t B, Hq, G, T, width;
   int32_t max_length;  // at most width << page_shift
+  // Work items (paged_plan.h).  A launch takes the rows with vectors_min to vectors_max query vectors a KV head;
+  // from 0 on, the rows without any too.
+  int32_t vectors_min, vectors_max;
+  int32_t tile, min_groups, target;
+  float *part_o;  // [item][tile][D] unnormalised outputs of rows cut into runs
+  float *part_ml;  // [item][tile][2] running maximum (log2 units) and sum
 };
 
 }  // namespace xattn

@@ -1,0 +1,415 @@
+// Attention over the paged 4-bit cache for rows of few query vectors a KV head: single tokens and short runs of them.
+//
+// A block of 8 waves takes an item (paged_plan.h): up to 16 * NC query vectors of a (row, KV head) over a run of
+// keys, one 64-key group at a time per wave.  A wave keeps the running maximum and sum of the softmax and its
+// output in registers; the waves meet in LDS at the end, runs in the merge kernel.
+//
+// Scores are S^T = K Q^T on the scaled matrix cores straight from the cache's codes (paged_mfma.h): row m of tile t
+// (of four) is key 4 m + t of the group, so a lane's four keys have their scales in one word and the instruction picks
+// the byte.  Lane (column q, g = lane / 16) then holds the scores of keys 16 g .. 16 g + 15 of its query: the softmax
+// needs two exchanges for the maximum, and the weights are the PV product's B operand where they are.  That
+// product's A operand is V^T: a value's codes become bf16 (exact, one conversion a pair) and pass through LDS,
+// half a group at a time, to be read transposed.
+//
+// Weights are rounded to bf16.  With up to 8 vectors the other 8 columns hold what that rounding loses
+// (w - bf16(w)), at no further matrix work, which leaves 2^-17 of a weight; with more the rounding is up to 2^-9.
+#include "paged_mfma.h"
+#include "paged_plan.h"
+#include "launch.h"
+
+namespace xattn {
+
+constexpr int kPagedWaves = 8, kPagedThreads = 64 * kPagedWaves;
+constexpr float kLowest = -3.0e38f;  // running maximum before any key
+
+template <int D>
+struct PagedShape {
+  static constexpr int KC = D == 256 ? 2 : 1;      // 128-feature chunks of a key (D = 64: half a chunk)
+  static constexpr int KL = D == 64 ? 2 : 4 * KC;  // 16-byte loads a lane makes of a group's keys
+  static constexpr int VL = D / 64;                // and of half a group's values
+  static constexpr int DT = D / 16;                // 16-feature tiles of the output
+  static constexpr int ROW = 2 * D, STAGE = 32 * ROW;
+};
+
+// Slot of 16-byte chunk c of staged row r.  The XOR spreads what one LDS pass serves over all banks: the stores of 8
+// consecutive rows (one chunk each) and the transposing reads of rows 8 g + 4 s + 0..3, g = 0..3 (a pair of chunks
+// each).
+template <int D>
+__device__ __forceinline__ int stage_swizzle(int r) {
+  return D == 64 ? 2 * (((r >> 1) & 1) + 2 * ((r >> 3) & 1)) ^ ((r >> 2) & 1)
+                 : 2 * ((r & 3) + 4 * ((r >> 3) & 1)) ^ ((r >> 2) & 1);
+}
+
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ u32x2 read_transposed(uint32_t lds) {
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4 *)(lds)));
+}
+
+// A lane's loads of a 64-key group and KV head, and its places in the staged half group.  A lane's offsets are few
+// words kept for the whole item, from which every address of an iteration follows by a constant.
+template <int D>
+struct GroupLoads {
+  using S = PagedShape<D>;
+  u32x4 k[S::KL];
+  uint32_t ks[S::KC];
+  u32x4 v[2][S::VL];
+  uint32_t vs[2][S::VL];
+  uint32_t key_at, key_scale_at, value_at, value_scale_at;  // in a group's codes and scales
+  uint32_t put_at, get_at;                                  // LDS bytes
+
+  __device__ __forceinline__ void init(int size, uint32_t stage, int m, int g) {
+    // Keys: load i of D = 64 takes key 4 m + 2 (g / 2) + i, block g % 2; else key 4 m + i / KC, block 4 (i % KC) + g.
+    key_at = D == 64 ? (4 * m + 2 * (g >> 1)) * 32 + 16 * (g & 1) : 4 * m * (D / 2) + 16 * g;
+    key_scale_at = (D == 64 ? (g & 1) : g) * size + 4 * m;
+    // Values: load w of half u takes row r of the half, key 16 (r / 8) + 8 u + r % 8.
+    const int r = D == 64 ? 16 * (g >> 1) + m : m, block = D == 64 ? (g & 1) : g, key = 16 * (r >> 3) + (r & 7);
+    value_at = key * (D / 2) + 16 * block;
+    value_scale_at = block * size + key;
+    put_at = stage + r * S::ROW + ((4 * block) ^ stage_swizzle<D>(r)) * 16;
+    const int x = 8 * g + (m >> 2);
+    get_at = stage + x * S::ROW + (((m & 3) >> 1) ^ stage_swizzle<D>(x)) * 16 + 8 * (m & 1);
+  }
+  // Keeps the compiler from carrying every address of the loop in a register of its own.
+  __device__ __forceinline__ void renew() {
+    asm volatile("" : "+v"(key_at), "+v"(key_scale_at), "+v"(value_at), "+v"(value_scale_at), "+v"(put_at), "+v"(get_at));
+  }
+
+  __device__ __forceinline__ void keys(const PagedArgs &a, int page, int h, int at) {
+    const int size = 1 << a.cache.page_shift;
+    const int64_t head = (int64_t)page * a.cache.Hkv + h;
+    const uint8_t *const codes = a.cache.key + (head * size + at) * (D / 2);
+    const uint8_t *const scales = a.cache.key_scale + head * (D / 32) * size + at;
+#pragma unroll
+    for (int i = 0; i < S::KL; ++i)
+      k[i] = *as_global(reinterpret_cast<const u32x4 *>(codes + (i / S::KC) * (D / 2) + (i % S::KC) * 64 + key_at));
+#pragma unroll
+    for (int c = 0; c < S::KC; ++c)
+      ks[c] = *as_global(reinterpret_cast<const uint32_t *>(scales + 4 * c * size + key_scale_at));
+  }
+  __device__ __forceinline__ void values(const PagedArgs &a, int page, int h, int at) {
+    const int size = 1 << a.cache.page_shift;
+    const int64_t head = (int64_t)page * a.cache.Hkv + h;
+    const uint8_t *const codes = a.cache.value + (head * size + at) * (D / 2);
+    const uint8_t *const scales = a.cache.value_scale + head * (D / 32) * size + at;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int w = 0; w < S::VL; ++w) {
+        const int key = 32 * (w / S::KC) + 8 * u, c = w % S::KC;
+        v[u][w] = *as_global(reinterpret_cast<const u32x4 *>(codes + key * (D / 2) + 64 * c + value_at));
+        vs[u][w] = *as_global(scales + 4 * c * size + key + value_scale_at);
+      }
+  }
+  // Half u's values into LDS as bf16.
+  __device__ __forceinline__ void put(int u) const {
+#pragma unroll
+    for (int w = 0; w < S::VL; ++w) {
+      const float scale = kv4_scale_value(min((int)vs[u][w], kKv4MaxScale));
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        *(__attribute__((address_space(3))) u32x4 *)((put_at ^ (16 * c)) + 16 * (w / S::KC) * S::ROW + 256 * (w % S::KC)) =
+            kv4_values(v[u][w][c], scale);
+    }
+  }
+  // Features 16 d .. of the staged half: this lane's feature of keys 16 g + 8 u + 0..7.
+  __device__ __forceinline__ bf16x8 get(int d) const {
+    const u32x2 x = read_transposed(get_at ^ (32 * d)), y = read_transposed((get_at ^ (32 * d + 16)) + 4 * S::ROW);
+    return as_bf16x8(u32x4{x.x, x.y, y.x, y.y});
+  }
+};
+
+// A query column's operands: the two e4m3 terms of each chunk, their scale bytes (terms' in bytes 0 and 1).
+template <int D>
+struct QueryOperand {
+  using S = PagedShape<D>;
+  u32x4 first[S::KC][2], second[S::KC][2];
+  int scale[S::KC];
+  __device__ __forceinline__ void load(const uint16_t *q, bool there, int m, int g) {
+#pragma unroll
+    for (int c = 0; c < S::KC; ++c) {
+      constexpr int PIECES = D == 64 ? 1 : 2;
+      uint32_t top[2] = {0, 0};
+      u32x4 x[2][2];
+#pragma unroll
+      for (int p = 0; p < PIECES; ++p) {
+        const uint16_t *const at = q + 128 * c + 64 * p + 16 * g;
+        x[p][0] = there ? load16(at) : u32x4{0, 0, 0, 0};
+        x[p][1] = there ? load16(at + 8) : u32x4{0, 0, 0, 0};
+        top[p] = largest(x[p][1], largest(x[p][0], 0u));
+        // The block's other 16 features are in lane group g ^ 1.
+        const auto r = __builtin_amdgcn_permlane16_swap(top[p], top[p], false, false);
+        top[p] = max(r[0], r[1]);
+      }
+      const int s0 = query_scale(top[0]), s1 = query_scale(top[1]);
+      split_query(x[0][0], x[0][1], s0, first[c][0], second[c][0]);
+      if constexpr (D == 64) first[c][1] = second[c][1] = u32x4{0, 0, 0, 0};
+      else split_query(x[1][0], x[1][1], s1, first[c][1], second[c][1]);
+      // Block g's scale is with lane group 2 (g % 2), of its first piece for g < 2.
+      const int from = m + 32 * (g & 1), b0 = __shfl(s0, from), b1 = __shfl(s1, from);
+      const int s = D == 64 || g < 2 ? b0 : b1;
+      scale[c] = s | (s == 255 ? 255 : s - 4) << 8;
+    }
+  }
+};
+
+template <int D, int NC>
+__global__ void __launch_bounds__(kPagedThreads, D == 256 || NC == 2 ? 2 : 4) paged_decode_kernel(const PagedArgs a) {
+  using S = PagedShape<D>;
+  constexpr int COLS = 16 * NC;
+  __shared__ __attribute__((aligned(1024))) char smem[kPagedWaves * S::STAGE];
+  __shared__ float2 wave_ml[kPagedWaves][16];
+  const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  PagedItem it;
+  if (!paged_item(a, blockIdx.x, it)) return;
+  if (it.count < a.T) paged_zero_padded<D, kPagedThreads>(a, it);
+  if (it.count == 0) return;
+  const int vectors = min(it.count * a.G - it.tile * COLS, COLS);
+  const bool twice = NC == 1 && vectors <= 8;  // columns 8..15 repeat the queries and take the weights' rests
+
+  QueryOperand<D> q[NC];
+  int last_key[NC];  // the last key that this lane's query sees
+#pragma unroll
+  for (int n = 0; n < NC; ++n) {
+    const int column = twice ? m & 7 : m + 16 * n, j = it.tile * COLS + column, t = j / a.G;
+    const bool there = column < vectors;
+    q[n].load(a.q.p + it.row * a.q.sb + (it.h * a.G + (j - t * a.G)) * a.q.sh + t * a.q.st, there, m, g);
+    last_key[n] = there ? it.length - it.count + t : -1;
+  }
+  const int all_see = it.length - it.count + it.tile * COLS / a.G;  // every query sees keys up to this one
+
+  f32x4 o[NC][S::DT];
+  float top[NC], sum[NC];
+#pragma unroll
+  for (int n = 0; n < NC; ++n) {
+    top[n] = kLowest;
+    sum[n] = 0.0f;
+#pragma unroll
+    for (int d = 0; d < S::DT; ++d) o[n][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  char *const stage = smem + wave * S::STAGE;
+
+  const int shift = a.cache.page_shift - 6;  // pages by groups
+  typedef const __attribute__((address_space(4))) int32_t *table_ptr;
+  const table_ptr table = (table_ptr)(a.table + (int64_t)it.row * a.width);
+  auto page_of = [&](int group) {
+    const int page = group < it.group_end ? table[group >> shift] : -1;
+    return page >= 0 && page < a.cache.pages ? page : -1;
+  };
+  auto place = [&](int group) { return (group & ((1 << shift) - 1)) * kGroupKeys; };
+
+  // A group's loads are under way while the one before it is worked on, its page number while the one before that is.
+  // Absent pages, and groups past the run, read page 0 and hide every key: no branch parts a group's work, which
+  // would have the compiler keep two groups in registers.
+  GroupLoads<D> in;
+  in.init(1 << a.cache.page_shift, (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)stage, m, g);
+  int group = it.group_begin + wave, page = page_of(group), next_page = page_of(group + kPagedWaves);
+  if (group < it.group_end) {
+    in.keys(a, max(page, 0), it.h, place(group));
+    in.values(a, max(page, 0), it.h, place(group));
+  }
+  for (; group < it.group_end; group += kPagedWaves) {
+    in.renew();
+    const int next = group + kPagedWaves, after_page = page_of(next + kPagedWaves), load_page = max(next_page, 0);
+    f32x4 s[NC][4];
+    const f32x4 zero{0.0f, 0.0f, 0.0f, 0.0f};
+    // A scale beside a zero operand (D = 64: one half of the lanes) has to be finite.
+    const int low = D == 64 ? (g < 2 ? (int)in.ks[0] : 0x7f7f7f7f) : 0, high = D == 64 ? (g < 2 ? 0x7f7f7f7f : (int)in.ks[0]) : 0;
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+      if constexpr (D == 64) {
+        const u32x4 none{0, 0, 0, 0};
+        const u32x4 f1[2] = {none, q[n].first[0][0]}, r1[2] = {none, q[n].second[0][0]};
+        const int ql = g < 2 ? q[n].scale[0] : 0x7f7f, qh = g < 2 ? 0x7f7f : q[n].scale[0];
+        s[n][0] = mfma16_fp4<0, 1>(in.k[0], q[n].second[0], mfma16_fp4<0, 0>(in.k[0], q[n].first[0], zero, low, ql), low, ql);
+        s[n][1] = mfma16_fp4<1, 1>(in.k[1], q[n].second[0], mfma16_fp4<1, 0>(in.k[1], q[n].first[0], zero, low, ql), low, ql);
+        s[n][2] = mfma16_fp4<2, 1>(in.k[0], r1, mfma16_fp4<2, 0>(in.k[0], f1, zero, high, qh), high, qh);
+        s[n][3] = mfma16_fp4<3, 1>(in.k[1], r1, mfma16_fp4<3, 0>(in.k[1], f1, zero, high, qh), high, qh);
+      } else {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) s[n][t] = zero;
+#pragma unroll
+        for (int c = 0; c < S::KC; ++c) {
+          const int qs = q[n].scale[c], ks = (int)in.ks[c];
+          s[n][0] = mfma16_fp4<0, 1>(in.k[c], q[n].second[c], mfma16_fp4<0, 0>(in.k[c], q[n].first[c], s[n][0], ks, qs), ks, qs);
+          s[n][1] = mfma16_fp4<1, 1>(in.k[S::KC + c], q[n].second[c],
+                                     mfma16_fp4<1, 0>(in.k[S::KC + c], q[n].first[c], s[n][1], ks, qs), ks, qs);
+          s[n][2] = mfma16_fp4<2, 1>(in.k[2 * S::KC + c], q[n].second[c],
+                                     mfma16_fp4<2, 0>(in.k[2 * S::KC + c], q[n].first[c], s[n][2], ks, qs), ks, qs);
+          s[n][3] = mfma16_fp4<3, 1>(in.k[3 * S::KC + c], q[n].second[c],
+                                     mfma16_fp4<3, 0>(in.k[3 * S::KC + c], q[n].first[c], s[n][3], ks, qs), ks, qs);
+        }
+      }
+    }
+    // The scores are taken here, before the registers of their keys are loaded anew.
+#pragma unroll
+    for (int n = 0; n < NC; ++n) asm volatile("" : "+v"(s[n][0]), "+v"(s[n][1]), "+v"(s[n][2]), "+v"(s[n][3]) : : "memory");
+    in.keys(a, load_page, it.h, place(next));
+    __builtin_amdgcn_sched_barrier(0);
+
+    // Weights: s[n][t][i] is key 16 g + 4 i + t of the group.
+    uint32_t pw[NC][2][4];
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+      if (group * kGroupKeys + kGroupKeys - 1 > all_see || page < 0) {
+        const int key = group * kGroupKeys + 16 * g, last = page < 0 ? -1 : last_key[n];
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[n][t][i] = key + 4 * i + t <= last ? s[n][t][i] : -INFINITY;
+      }
+      float x = fmaxf(fmaxf(s[n][0][0], s[n][1][0]), fmaxf(s[n][2][0], s[n][3][0]));
+#pragma unroll
+      for (int i = 1; i < 4; ++i) x = fmaxf(x, fmaxf(fmaxf(s[n][0][i], s[n][1][i]), fmaxf(s[n][2][i], s[n][3][i])));
+      x = pair_max32(pair_max16(x));
+      const float now = fmaxf(top[n], x * a.scale_log2);
+      if (__any(now > top[n])) {
+        const float keep = fast_exp2(top[n] - now);
+        sum[n] *= keep;
+#pragma unroll
+        for (int d = 0; d < S::DT; ++d) o[n][d] *= keep;
+        top[n] = now;
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const int i = 2 * u + w / 2, t = 2 * (w & 1);
+          const float p0 = fast_exp2(fmaf(s[n][t][i], a.scale_log2, -now)), p1 = fast_exp2(fmaf(s[n][t + 1][i], a.scale_log2, -now));
+          sum[n] += p0 + p1;
+          const uint32_t word = pack_bf16x2(p0, p1);
+          pw[n][u][w] = twice && m >= 8 ? pack_bf16x2(p0 - bf16_lo(word), p1 - bf16_hi(word)) : word;
+        }
+    }
+
+    __builtin_amdgcn_sched_barrier(0);
+    // Output: half the group's values in LDS at a time, read transposed.
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      in.put(u);
+      if (u == 1) in.values(a, load_page, it.h, place(next));
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int d = 0; d < S::DT; ++d) {
+        if (d % 4 == 0) __builtin_amdgcn_sched_barrier(0);
+        const bf16x8 v = in.get(d);
+#pragma unroll
+        for (int n = 0; n < NC; ++n)
+          o[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+              v, as_bf16x8(u32x4{pw[n][u][0], pw[n][u][1], pw[n][u][2], pw[n][u][3]}), o[n][d], 0, 0, 0);
+      }
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    page = next_page, next_page = after_page;
+  }
+
+  // The waves' outputs, and the weights' rests (columns 8..15), meet in LDS.
+#pragma unroll
+  for (int n = 0; n < NC; ++n) {
+    const float l = pair_sum32(pair_sum16(sum[n]));
+    if (twice) {
+#pragma unroll
+      for (int d = 0; d < S::DT; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[n][d][i] += dpp_move<kDppRowRor8>(o[n][d][i]);
+    }
+    __syncthreads();
+    const int columns = min(vectors - 16 * n, 16);
+    if (g == 0) wave_ml[wave][m] = float2{top[n], l};
+    if (m < columns) {
+#pragma unroll
+      for (int d = 0; d < S::DT; ++d)
+        *reinterpret_cast<f32x4 *>(stage + m * (4 * D) + ((4 * d + g) ^ (m & 7)) * 16) = o[n][d];
+    }
+    __syncthreads();
+    for (int i = tid; i < columns * (D / 4); i += kPagedThreads) {
+      const int column = i / (D / 4), f = i - column * (D / 4);
+      float best = kLowest, total = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kPagedWaves; ++w) best = fmaxf(best, wave_ml[w][column].x);
+      f32x4 out{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int w = 0; w < kPagedWaves; ++w) {
+        const float2 ml = wave_ml[w][column];
+        const float keep = fast_exp2(ml.x - best);
+        total += ml.y * keep;
+        out += *reinterpret_cast<const f32x4 *>(smem + w * S::STAGE + column * (4 * D) + (f ^ (column & 7)) * 16) * keep;
+      }
+      if (it.nsplit > 1) {
+        const int64_t record = (int64_t)blockIdx.x * COLS + 16 * n + column;
+        *as_global(reinterpret_cast<f32x4 *>(a.part_o + record * D + 4 * f)) = out;
+        if (f == 0) *as_global(reinterpret_cast<f32x2 *>(a.part_ml + 2 * record)) = f32x2{best, total};
+      } else {
+        const int j = it.tile * COLS + 16 * n + column, t = j / a.G;
+        const float by = total == 0.0f ? 0.0f : 1.0f / total;
+        out *= by;
+        *as_global(reinterpret_cast<u32x2 *>(
+            a.out + (((int64_t)it.row * a.T + t) * a.Hq + it.h * a.G + (j - t * a.G)) * D + 4 * f)) =
+            u32x2{pack_bf16x2(out[0], out[1]), pack_bf16x2(out[2], out[3])};
+      }
+    }
+  }
+}
+
+// Joins the runs of a (row, KV head, tile) of either launch (blockIdx.z).
+template <int D>
+__global__ void __launch_bounds__(256) paged_merge_kernel(const PagedArgs few, const PagedArgs many) {
+  const PagedArgs &a = blockIdx.z == 0 ? few : many;
+  const int tile = blockIdx.x / a.cache.Hkv, h = blockIdx.x - tile * a.cache.Hkv;
+  PagedItem it;
+  paged_row_items(a, blockIdx.y, it);
+  if (it.nsplit <= 1 || tile >= it.tiles) return;
+  const int vectors = min(it.count * a.G - tile * a.tile, a.tile);
+  for (int i = threadIdx.x; i < vectors * (D / 4); i += 256) {
+    const int column = i / (D / 4), f = i - column * (D / 4);
+    float best = kLowest, total = 0.0f;
+    f32x4 out{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s = 0; s < it.nsplit; ++s) {
+      const int64_t record = ((int64_t)it.begin + (int64_t)(tile * it.nsplit + s) * a.cache.Hkv + h) * a.tile + column;
+      const f32x2 ml = *as_global(reinterpret_cast<const f32x2 *>(a.part_ml + 2 * record));
+      const f32x4 part = *as_global(reinterpret_cast<const f32x4 *>(a.part_o + record * D + 4 * f));
+      const float now = fmaxf(best, ml.x), old = fast_exp2(best - now), keep = fast_exp2(ml.x - now);
+      best = now;
+      total = total * old + ml.y * keep;
+      out = out * old + part * keep;
+    }
+    const int j = tile * a.tile + column, t = j / a.G;
+    const float by = total == 0.0f ? 0.0f : 1.0f / total;
+    out *= by;
+    *as_global(reinterpret_cast<u32x2 *>(
+        a.out + (((int64_t)it.row * a.T + t) * a.Hq + h * a.G + (j - t * a.G)) * D + 4 * f)) =
+        u32x2{pack_bf16x2(out[0], out[1]), pack_bf16x2(out[2], out[3])};
+  }
+}
+
+template <int D>
+static void launch_decode_d(const PagedArgs &a, unsigned items, hipStream_t stream) {
+  if constexpr (paged_decode_columns(D) == 32) {
+    if (a.tile == 32) hipLaunchKernelGGL((paged_decode_kernel<D, 2>), dim3(items), dim3(kPagedThreads), 0, stream, a);
+  }
+  if (a.tile == 16) hipLaunchKernelGGL((paged_decode_kernel<D, 1>), dim3(items), dim3(kPagedThreads), 0, stream, a);
+}
+
+hipError_t launch_paged_decode(const PagedArgs &a, unsigned items, hipStream_t stream) {
+  switch (a.cache.D) {
+    case 64: launch_decode_d<64>(a, items, stream); break;
+    case 128: launch_decode_d<128>(a, items, stream); break;
+    default: launch_decode_d<256>(a, items, stream); break;
+  }
+  return hipGetLastError();
+}
+
+hipError_t launch_paged_merge(const PagedArgs &few, const PagedArgs *many, int tiles, hipStream_t stream) {
+  const dim3 grid(tiles * few.cache.Hkv, few.B, many ? 2 : 1);
+  const PagedArgs &other = many ? *many : few;
+  switch (few.cache.D) {
+    case 64: hipLaunchKernelGGL((paged_merge_kernel<64>), grid, dim3(256), 0, stream, few, other); break;
+    case 128: hipLaunchKernelGGL((paged_merge_kernel<128>), grid, dim3(256), 0, stream, few, other); break;
+    default: hipLaunchKernelGGL((paged_merge_kernel<256>), grid, dim3(256), 0, stream, few, other); break;
+  }
+  return hipGetLastError();
+}
+
+}  // namespace xattn

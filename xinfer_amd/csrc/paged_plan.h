@@ -1,0 +1,136 @@
+// Work items of attention over the paged cache, laid out on the device from the rows' lengths.
+//
+// A launch is sized by the shapes alone.  Its waves each compute the same plan from the lengths: a row's keys are
+// cut into `nsplit` runs of 64-key groups, its query vectors (query heads of a KV head times tokens) into tiles, and
+// an item is a (tile, run, KV head).  Runs take at least `min_groups` groups, and as many more as leave about
+// `target` items, so a few long rows fill the chip and many rows are not cut at all.  Items past the plan's last end
+// at once.  The KV head counts fastest: consecutive blocks go to the 8 XCDs in turn, so with 8 KV heads the tiles
+// of one head meet in one XCD's L2.
+#pragma once
+
+#include "kv4_device.h"
+
+namespace xattn {
+
+constexpr int kGroupKeys = 64;
+
+struct PagedRow {
+  int count, length;
+};
+__device__ __forceinline__ PagedRow paged_row(const PagedArgs &a, int r) {
+  PagedRow p;
+  p.count = min(max(a.lengths[r], 0), min(a.T, a.max_length));
+  p.length = min(max(a.lengths[a.B + r], p.count), a.max_length);
+  return p;
+}
+
+struct PagedItem {
+  int row, count, length;
+  int h, tile, split, nsplit, tiles;
+  int group_begin, group_end;  // 64-key groups of the run
+  int begin;                   // the row's first item
+};
+
+// What a launch takes of row r: 64-key groups and tiles; no tiles: the row is another launch's.
+struct PagedShare {
+  int groups, tiles;
+};
+__device__ __forceinline__ PagedShare paged_share(const PagedArgs &a, const PagedRow &p) {
+  const int vectors = p.count * a.G;
+  PagedShare s{0, 0};
+  if (vectors == 0) {
+    s.tiles = a.vectors_min == 0 ? 1 : 0;  // only zeros to write
+  } else if (vectors >= a.vectors_min && vectors <= a.vectors_max) {
+    s.groups = (p.length + kGroupKeys - 1) / kGroupKeys;
+    s.tiles = (vectors + a.tile - 1) / a.tile;
+  }
+  return s;
+}
+
+// Groups of a run at most.
+__device__ __forceinline__ int paged_run(const PagedArgs &a) {
+  const int lane = threadIdx.x & 63;
+  float total = 0.0f;
+  for (int base = 0; base < a.B; base += 64) {
+    PagedShare s{0, 0};
+    if (base + lane < a.B) s = paged_share(a, paged_row(a, base + lane));
+    total += (float)s.groups * (float)s.tiles;
+  }
+  total = group_sum<64>(total) * (float)a.cache.Hkv;
+  return max(a.min_groups, (int)(total / (float)a.target) + 1);
+}
+__device__ __forceinline__ int paged_splits(const PagedShare &s, int run) { return max(1, (s.groups + run - 1) / run); }
+
+// Item `index` of the plan; false past its last.  Every lane of a wave calls it, with the same index.
+__device__ __forceinline__ bool paged_item(const PagedArgs &a, int index, PagedItem &it) {
+  const int lane = threadIdx.x & 63, run = paged_run(a), Hkv = a.cache.Hkv;
+  int before = 0;
+  for (int base = 0; base < a.B; base += 64) {
+    PagedRow p{0, 0};
+    PagedShare s{0, 0};
+    if (base + lane < a.B) {
+      p = paged_row(a, base + lane);
+      s = paged_share(a, p);
+    }
+    const int nsplit = paged_splits(s, run), items = s.tiles * nsplit * Hkv, upto = before + wave_scan(items);
+    const uint64_t past = __ballot(upto > index);
+    if (past != 0) {
+      const int at = __builtin_ctzll(past);
+      it.row = base + at;
+      it.count = __builtin_amdgcn_readlane(p.count, at);
+      it.length = __builtin_amdgcn_readlane(p.length, at);
+      it.nsplit = __builtin_amdgcn_readlane(nsplit, at);
+      it.tiles = __builtin_amdgcn_readlane(s.tiles, at);
+      it.begin = __builtin_amdgcn_readlane(upto - items, at);
+      const int groups = __builtin_amdgcn_readlane(s.groups, at);
+      const int i = index - it.begin, rest = i / Hkv;
+      it.h = i - rest * Hkv;
+      it.tile = rest / it.nsplit;
+      it.split = rest - it.tile * it.nsplit;
+      it.group_begin = (int)((int64_t)groups * it.split / it.nsplit);
+      it.group_end = (int)((int64_t)groups * (it.split + 1) / it.nsplit);
+      return true;
+    }
+    before = __builtin_amdgcn_readlane(upto, 63);
+  }
+  return false;
+}
+
+// Row `row`'s part of the plan: its first item, splits and tiles.
+__device__ __forceinline__ void paged_row_items(const PagedArgs &a, int row, PagedItem &it) {
+  const int lane = threadIdx.x & 63, run = paged_run(a), Hkv = a.cache.Hkv;
+  int before = 0;
+  for (int base = 0; base <= row; base += 64) {
+    PagedRow p{0, 0};
+    PagedShare s{0, 0};
+    if (base + lane < a.B) {
+      p = paged_row(a, base + lane);
+      s = paged_share(a, p);
+    }
+    const int nsplit = paged_splits(s, run), items = s.tiles * nsplit * Hkv, upto = before + wave_scan(items);
+    if (row < base + 64) {
+      const int at = row - base;
+      it.row = row;
+      it.count = __builtin_amdgcn_readlane(p.count, at);
+      it.length = __builtin_amdgcn_readlane(p.length, at);
+      it.nsplit = __builtin_amdgcn_readlane(nsplit, at);
+      it.tiles = __builtin_amdgcn_readlane(s.tiles, at);
+      it.begin = __builtin_amdgcn_readlane(upto - items, at);
+    }
+    before = __builtin_amdgcn_readlane(upto, 63);
+  }
+}
+
+// Zeros for the row's padded queries of the item's head, by the item of its first tile and run.
+template <int D, int THREADS>
+__device__ __forceinline__ void paged_zero_padded(const PagedArgs &a, const PagedItem &it) {
+  if (it.tile != 0 || it.split != 0) return;
+  constexpr int CHUNKS = D / 8;
+  uint16_t *const out = a.out + ((int64_t)it.row * a.T * a.Hq + (int64_t)it.h * a.G) * D;
+  for (int i = threadIdx.x / CHUNKS; i < (a.T - it.count) * a.G; i += THREADS / CHUNKS) {
+    const int t = i / a.G;
+    store16(out + ((int64_t)(it.count + t) * a.Hq + (i - t * a.G)) * D + 8 * (threadIdx.x % CHUNKS), u32x4{0, 0, 0, 0});
+  }
+}
+
+}  // namespace xattn

@@ -1,0 +1,261 @@
+// Attention over the paged 4-bit cache for rows of many query vectors a KV head: prompt chunks.
+//
+// A block of 4 waves takes an item (paged_plan.h): 128 query vectors of a (row, KV head), 32 a wave, over a run of
+// keys in 64-key groups.  A wave reads the group's keys as they lie in the cache, as the A operand of the scaled
+// 32x32x64 product against its queries' two e4m3 terms (paged_mfma.h): row m of tile t (of two) is key 2 m + t, so a
+// lane's two keys have their scales in neighbouring bytes.  A lane (column q, half h) then holds 32 scores of its query,
+// and for each 16 keys 8 neighbouring ones, which is the B operand of the bf16 PV product: nothing of the softmax
+// crosses lanes but the maximum and, at the end, the sum of the two halves.
+//
+// The block turns the group's values into bf16 (exact) in LDS together, one group ahead, and every wave reads
+// them transposed as the A operand.  One barrier a group.
+//
+// Weights are rounded to bf16 (2^-9 of a weight at most, on average lost in the sum); their sum is taken before.
+#include "paged_mfma.h"
+#include "paged_plan.h"
+#include "launch.h"
+
+namespace xattn {
+
+constexpr int kChunkWaves = 4, kChunkThreads = 64 * kChunkWaves;
+constexpr float kLowestMax = -3.0e38f;  // running maximum before any key
+
+template <int D>
+struct ChunkShape {
+  static constexpr int KS = D / 64;                                  // 64-feature steps of the scores
+  static constexpr int DT = D / 32;                                  // 32-feature tiles of the output
+  static constexpr int ROW = 2 * D, STAGE = 64 * ROW;                // staged values of a group
+  static constexpr int UNITS = 64 * (D / 32);                        // (key, block) units of a group
+  static constexpr int VL = (UNITS + kChunkThreads - 1) / kChunkThreads;
+};
+
+// XOR of the 16-byte chunk index of staged row r: the four rows that a half's transposing read takes lie in different
+// quarters of the banks, and so do the blocks and rows that eight storing lanes hold.
+template <int D>
+__device__ __forceinline__ int chunk_swizzle(int r) {
+  return D == 64 ? 5 * ((r >> 1) & 1) : 5 * (r & 3);
+}
+
+typedef short i16x4p __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ u32x2 lds_transposed(uint32_t lds) {
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4p *)(lds)));
+}
+
+template <int D>
+__global__ void __launch_bounds__(kChunkThreads, D == 256 ? 1 : 2) paged_prefill_kernel(const PagedArgs a) {
+  using S = ChunkShape<D>;
+  constexpr int COLS = 32 * kChunkWaves;
+  __shared__ __attribute__((aligned(1024))) char smem[2 * S::STAGE];
+  const int tid = threadIdx.x, lane = tid & 63, m = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  PagedItem it;
+  if (!paged_item(a, blockIdx.x, it)) return;
+  paged_zero_padded<D, kChunkThreads>(a, it);
+
+  // This wave's queries.
+  const int vectors = it.count * a.G, j = it.tile * COLS + 32 * wave + m;
+  const int t = j / a.G, head = it.h * a.G + (j - t * a.G);
+  const bool there = j < vectors;
+  const int last_key = there ? it.length - it.count + t : -1;
+  const int wave_first = it.tile * COLS + 32 * wave;
+  const int all_see = it.length - it.count + wave_first / a.G;  // all of the wave's queries see keys up to this one,
+  const int none_see = wave_first < vectors                     // and none of them this one or a later
+                           ? it.length - it.count + (min(wave_first + 32, vectors) - 1) / a.G + 1 : 0;
+  const int tile_end = it.length - it.count + (min(it.tile * COLS + COLS, vectors) - 1) / a.G + 1;
+  const int group_end = min(it.group_end, (tile_end + kGroupKeys - 1) / kGroupKeys);
+
+  u32x4 first[S::KS][2], second[S::KS][2];
+  int qscale[S::KS];
+  {
+    const uint16_t *const q = a.q.p + it.row * a.q.sb + head * a.q.sh + t * a.q.st;
+#pragma unroll
+    for (int s = 0; s < S::KS; ++s) {
+      int b[2];
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        const uint16_t *const at = q + 64 * s + 32 * p + 16 * h;
+        const u32x4 x0 = there ? load16(at) : u32x4{0, 0, 0, 0}, x1 = there ? load16(at + 8) : u32x4{0, 0, 0, 0};
+        const uint32_t top = largest(x1, largest(x0, 0u));
+        const auto r = __builtin_amdgcn_permlane32_swap(top, top, false, false);  // the block's other half
+        b[p] = query_scale(max(r[0], r[1]));
+        split_query(x0, x1, b[p], first[s][p], second[s][p]);
+      }
+      const int mine = h == 0 ? b[0] : b[1];
+      qscale[s] = mine | (mine == 255 ? 255 : mine - 4) << 8;
+    }
+  }
+
+  f32x16 o[S::DT];
+#pragma unroll
+  for (int d = 0; d < S::DT; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[d][r] = 0.0f;
+  float top = kLowestMax, sum = 0.0f;
+
+  const int shift = a.cache.page_shift - 6, size = 1 << a.cache.page_shift;
+  typedef const __attribute__((address_space(4))) int32_t *table_ptr;
+  const table_ptr table = (table_ptr)(a.table + (int64_t)it.row * a.width);
+  auto page_of = [&](int group) {
+    const int page = group < group_end ? table[group >> shift] : -1;
+    return page >= 0 && page < a.cache.pages ? page : -1;
+  };
+  auto place = [&](int group) { return (group & ((1 << shift) - 1)) * kGroupKeys; };
+
+  // Keys of a group: lane (m, h) holds keys 2 m + t, blocks 2 s + h.
+  u32x4 k[2][S::KS];
+  uint32_t ks[S::KS];
+  uint32_t key_at = 2 * m * (D / 2) + 16 * h, key_scale_at = h * size + 2 * m;
+  auto load_keys = [&](int group, int page) {
+    const int64_t hd = (int64_t)max(page, 0) * a.cache.Hkv + it.h;
+    const uint8_t *const codes = a.cache.key + (hd * size + place(group)) * (D / 2);
+    const uint8_t *const scales = a.cache.key_scale + hd * (D / 32) * size + place(group);
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int s = 0; s < S::KS; ++s)
+        k[x][s] = *as_global(reinterpret_cast<const u32x4 *>(codes + x * (D / 2) + 32 * s + key_at));
+#pragma unroll
+    for (int s = 0; s < S::KS; ++s) ks[s] = *as_global(reinterpret_cast<const uint16_t *>(scales + 2 * s * size + key_scale_at));
+  };
+  // Values of a group: unit w of a thread is (key, block) = tid + w * threads, the block counting fastest.
+  u32x4 v[S::VL];
+  uint32_t vs[S::VL];
+  const int block = tid % (D / 32), row0 = tid / (D / 32);
+  constexpr int ROWS = kChunkThreads / (D / 32);  // rows a load covers
+  const uint32_t value_at = row0 * (D / 2) + 16 * block, value_scale_at = block * size + row0;
+  const uint32_t stage0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)smem;
+  const bool stages = S::UNITS >= kChunkThreads || tid < S::UNITS;
+  const uint32_t put_at = stage0 + row0 * S::ROW + ((4 * block) ^ chunk_swizzle<D>(row0) ^ (block >> 2)) * 16;
+  auto load_values = [&](int group, int page) {
+    const int64_t hd = (int64_t)max(page, 0) * a.cache.Hkv + it.h;
+    const uint8_t *const codes = a.cache.value + (hd * size + place(group)) * (D / 2);
+    const uint8_t *const scales = a.cache.value_scale + hd * (D / 32) * size + place(group);
+    if (stages) {
+#pragma unroll
+      for (int w = 0; w < S::VL; ++w) {
+        v[w] = *as_global(reinterpret_cast<const u32x4 *>(codes + w * ROWS * (D / 2) + value_at));
+        vs[w] = *as_global(scales + w * ROWS + value_scale_at);
+      }
+    }
+  };
+  auto put_values = [&](int buffer) {
+    if (stages) {
+#pragma unroll
+      for (int w = 0; w < S::VL; ++w) {
+        const float scale = kv4_scale_value(min((int)vs[w], kKv4MaxScale));
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          *(__attribute__((address_space(3))) u32x4 *)((put_at ^ (16 * c)) + w * ROWS * S::ROW + buffer * S::STAGE) =
+              kv4_values(v[w][c], scale);
+      }
+    }
+  };
+  // Transposing reads: lane (m, h) gets feature 32 d + m of keys 16 b + 8 h + 0..7.
+  const int x = 8 * h + ((lane & 15) >> 2);
+  const uint32_t get_at = stage0 + x * S::ROW + ((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ chunk_swizzle<D>(x)) * 16 + 8 * (lane & 1);
+
+  int group = it.group_begin;
+  if (group < group_end) {
+    int page = page_of(group), next_page = page_of(group + 1);
+    load_values(group, page);
+    load_keys(group, page);
+    put_values(0);
+    load_values(group + 1, next_page);
+    for (int buffer = 0; group < group_end; ++group, buffer ^= 1) {
+      asm volatile("" : "+v"(key_at), "+v"(key_scale_at));
+      const int after_page = page_of(group + 2);
+      // Every wave has stored its part of this group's values, and is done with the group before.
+      __syncthreads();
+      put_values(buffer ^ 1);
+      load_values(group + 2, after_page);
+      const bool active = group * kGroupKeys < none_see && page >= 0;  // uniform in the wave
+      f32x16 s[2];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[0][r] = s[1][r] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < S::KS; ++i) {
+        s[0] = mfma32_fp4<0, 0>(k[0][i], first[i], s[0], (int)ks[i], qscale[i]);
+        s[0] = mfma32_fp4<0, 1>(k[0][i], second[i], s[0], (int)ks[i], qscale[i]);
+        s[1] = mfma32_fp4<1, 0>(k[1][i], first[i], s[1], (int)ks[i], qscale[i]);
+        s[1] = mfma32_fp4<1, 1>(k[1][i], second[i], s[1], (int)ks[i], qscale[i]);
+      }
+      asm volatile("" : "+v"(s[0]), "+v"(s[1]) : : "memory");
+      load_keys(group + 1, next_page);
+      page = next_page, next_page = after_page;
+      if (!active) continue;
+      // s[x][r] is key 16 (r / 4) + 8 h + 2 (r % 4) + x of the group.
+      if (group * kGroupKeys + kGroupKeys - 1 > all_see) {
+        const int key = group * kGroupKeys + 8 * h;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int at = key + 16 * (r / 4) + 2 * (r % 4);
+          s[0][r] = at <= last_key ? s[0][r] : -INFINITY;
+          s[1][r] = at + 1 <= last_key ? s[1][r] : -INFINITY;
+        }
+      }
+      float best = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+      for (int r = 1; r < 16; ++r) best = fmaxf(best, fmaxf(s[0][r], s[1][r]));
+      best = fmaxf(top, pair_max32(best) * a.scale_log2);
+      if (__any(best > top)) {
+        const float keep = fast_exp2(top - best);
+        sum *= keep;
+#pragma unroll
+        for (int d = 0; d < S::DT; ++d) o[d] *= keep;
+        top = best;
+      }
+      const uint32_t get = get_at + buffer * S::STAGE;
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        uint32_t pw[4];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const float p0 = fast_exp2(fmaf(s[0][4 * b + w], a.scale_log2, -top)), p1 = fast_exp2(fmaf(s[1][4 * b + w], a.scale_log2, -top));
+          sum += p0 + p1;
+          pw[w] = pack_bf16x2(p0, p1);
+        }
+        const bf16x8 weights = as_bf16x8(u32x4{pw[0], pw[1], pw[2], pw[3]});
+#pragma unroll
+        for (int d = 0; d < S::DT; ++d) {
+          const uint32_t at = (get ^ (64 * d) ^ (d >= 4 ? 16 : 0)) + 16 * b * S::ROW;
+          const u32x2 lo = lds_transposed(at), hi = lds_transposed(at + 4 * S::ROW);
+          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(u32x4{lo.x, lo.y, hi.x, hi.y}), weights, o[d], 0, 0, 0);
+        }
+      }
+    }
+  }
+
+  sum = pair_sum32(sum);
+  if (!there) return;
+  // o[d][r] is feature 32 d + 8 (r / 4) + 4 h + r % 4.
+  if (it.nsplit > 1) {
+    const int64_t record = (int64_t)blockIdx.x * COLS + 32 * wave + m;
+#pragma unroll
+    for (int d = 0; d < S::DT; ++d)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        *as_global(reinterpret_cast<f32x4 *>(a.part_o + record * D + 32 * d + 8 * r + 4 * h)) =
+            f32x4{o[d][4 * r], o[d][4 * r + 1], o[d][4 * r + 2], o[d][4 * r + 3]};
+    if (h == 0) *as_global(reinterpret_cast<f32x2 *>(a.part_ml + 2 * record)) = f32x2{top, sum};
+  } else {
+    const float by = sum == 0.0f ? 0.0f : 1.0f / sum;
+    uint16_t *const out = a.out + (((int64_t)it.row * a.T + t) * a.Hq + head) * D + 4 * h;
+#pragma unroll
+    for (int d = 0; d < S::DT; ++d)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        *as_global(reinterpret_cast<u32x2 *>(out + 32 * d + 8 * r)) =
+            u32x2{pack_bf16x2(o[d][4 * r] * by, o[d][4 * r + 1] * by), pack_bf16x2(o[d][4 * r + 2] * by, o[d][4 * r + 3] * by)};
+  }
+}
+
+hipError_t launch_paged_prefill(const PagedArgs &a, unsigned items, hipStream_t stream) {
+  switch (a.cache.D) {
+    case 64: hipLaunchKernelGGL((paged_prefill_kernel<64>), dim3(items), dim3(kChunkThreads), 0, stream, a); break;
+    case 128: hipLaunchKernelGGL((paged_prefill_kernel<128>), dim3(items), dim3(kChunkThreads), 0, stream, a); break;
+    default: hipLaunchKernelGGL((paged_prefill_kernel<256>), dim3(items), dim3(kChunkThreads), 0, stream, a); break;
+  }
+  return hipGetLastError();
+}
+
+}  // namespace xattn
