@@ -28,8 +28,7 @@ LIBRARY_NAME = "libxinfer_attention_ops.so"
 ARCH = "gfx950"
 
 KERNEL_SOURCES = ("append.hip", "decode.hip", "prefill.hip", "prefill_d256.hip", "merge.hip", "norm_rope.hip",
-                  "gemv.hip", "scratch.hip", "kv4_cache.hip", "paged_reserve.hip", "paged_decode.hip",
-                  "paged_prefill.hip")
+                  "gemv.hip", "scratch.hip", "kv4_cache.hip", "paged_reserve.hip", "paged_attention.hip")
 HOST_SOURCES = ("capi.cpp", "kv4_capi.cpp")
 TORCH_SOURCES = ("torch_ops.cpp", "kv4_ops.cpp")
 

@@ -3,6 +3,7 @@
 #include <cmath>
 #include <cstdint>
 #include <limits>
+#include <cstdlib>
 
 #include "xinfer_attention.h"
 #include "kv4_common.h"
@@ -50,14 +51,7 @@ View view_of(const xinfer_view4 &t) {
   return View{static_cast<const uint16_t *>(t.data), t.stride[0], t.stride[1], t.stride[2]};
 }
 
-// Launches and workspace of a paged attention call, from the shapes and the bound on the lengths alone.  Rows of few
-// query vectors go to the decode kernel, the others, where the shapes allow any, to the prefill kernel.
-struct PagedLaunch {
-  PagedArgs a;
-  int64_t items;
-  int tiles;     // of a row and KV head, at most
-  size_t bytes;  // records of rows cut into runs; 0: no row can be
-};
+// Launches and workspace of a paged attention call come from the shapes and the bound on the lengths alone.
 constexpr int kPagedTarget = 512;  // items that fill the chip: two blocks a CU
 constexpr int kPagedDecodeGroups = 16, kPagedPrefillGroups = 8;
 
@@ -68,25 +62,22 @@ PagedLaunch paged_launch(const PagedArgs &shapes, int vectors_min, int vectors_m
   l.a.vectors_min = vectors_min;
   l.a.vectors_max = vectors_max;
   l.a.tile = tile;
+  int target = kPagedTarget;
+  if (const char *e = getenv(vectors_max > 32 ? "KV4_PG" : "KV4_DG")) min_groups = atoi(e);
+  if (const char *e = getenv(vectors_max > 32 ? "KV4_PT" : "KV4_DT")) target = atoi(e);
   l.a.min_groups = min_groups;
-  l.a.target = kPagedTarget;
+  l.a.target = target;
   l.tiles = (int)ceil_div(std::min<int64_t>((int64_t)shapes.T * shapes.G, vectors_max), tile);
   // A row and tile has at most one run more than its share of the target.
   const int64_t whole = (int64_t)shapes.B * shapes.cache.Hkv * l.tiles;
   const int64_t runs = ceil_div(ceil_div(shapes.max_length, 64), min_groups);
-  l.items = runs <= 1 ? whole : std::min(whole * runs, whole + kPagedTarget);
+  l.items = runs <= 1 ? whole : std::min(whole * runs, whole + target);
   l.bytes = runs <= 1 ? 0 : (size_t)l.items * tile * (shapes.cache.D + 2) * sizeof(float);
   return l;
 }
 
-struct PagedCall {
-  PagedLaunch few, many;
-  bool both;
-  size_t bytes() const { return few.bytes + (both ? many.bytes : 0); }
-};
-
 int paged_call(const xinfer_view4 &q, const xinfer_kv4_cache &cache, int64_t table_width, int64_t max_length,
-               PagedCall &call) {
+               PagedLaunches &call) {
   PagedArgs a{};
   if (!cache_of(cache, a.cache)) return XINFER_ERR_KV4_CACHE;
   const int64_t B = q.size[0], Hq = q.size[1], T = q.size[2];
@@ -104,8 +95,12 @@ int paged_call(const xinfer_view4 &q, const xinfer_kv4_cache &cache, int64_t tab
   a.max_length = (int32_t)(max_length == 0 ? capacity : std::min(max_length, capacity));
   const int columns = paged_decode_columns(a.cache.D), vectors = a.T * a.G;
   call.few = paged_launch(a, 0, vectors <= 32 ? 32 : columns, vectors <= 16 ? 16 : columns, kPagedDecodeGroups);
-  call.both = vectors > 32;
-  if (call.both) call.many = paged_launch(a, columns + 1, kIntMax, kPagedPrefillTile, kPagedPrefillGroups);
+  call.many = PagedLaunch{a, 0, 0, 0};
+  if (vectors > 32) {
+    // One row alone goes to the prefill kernel whatever its count.
+    call.many = paged_launch(a, B == 1 ? 0 : columns + 1, kIntMax, kPagedPrefillTile, kPagedPrefillGroups);
+    if (B == 1) call.few.items = call.few.bytes = 0;
+  }
   return XINFER_OK;
 }
 
@@ -220,7 +215,7 @@ int xinfer_qk_norm_rope_append_kv4(const xinfer_view4 *q, const xinfer_view4 *ke
 
 size_t xinfer_paged_attention_kv4_workspace_size(const xinfer_view4 *q, const xinfer_kv4_cache *cache,
                                                  int64_t table_width, int64_t max_length) {
-  PagedCall call{};
+  PagedLaunches call{};
   if (!q || !cache || paged_call(*q, *cache, table_width, max_length, call) != XINFER_OK) return 0;
   return call.bytes();
 }
@@ -229,7 +224,7 @@ int xinfer_paged_attention_kv4(const xinfer_view4 *q, const xinfer_kv4_cache *ca
                                int64_t table_width, const int32_t *lengths, int64_t max_length, double scale,
                                void *out, void *workspace, size_t workspace_bytes, void *stream) {
   if (!q || !cache) return XINFER_ERR_ARGUMENT;
-  PagedCall call{};
+  PagedLaunches call{};
   const int status = paged_call(*q, *cache, table_width, max_length, call);
   if (status != XINFER_OK) return status;
   if (!(std::isfinite(scale) && scale > 0)) return XINFER_ERR_SCALE;
@@ -248,13 +243,7 @@ int xinfer_paged_attention_kv4(const xinfer_view4 *q, const xinfer_kv4_cache *ca
     l->a.part_ml = l->a.part_o + l->items * l->a.tile * l->a.cache.D;
     records += l->bytes;
   }
-  const hipStream_t on = static_cast<hipStream_t>(stream);
-  if (call.both && launch_paged_prefill(call.many.a, (unsigned)call.many.items, on) != hipSuccess)
-    return XINFER_ERR_LAUNCH;
-  if (launch_paged_decode(call.few.a, (unsigned)call.few.items, on) != hipSuccess) return XINFER_ERR_LAUNCH;
-  if (call.bytes() == 0) return XINFER_OK;
-  return done(launch_paged_merge(call.few.a, call.both ? &call.many.a : nullptr,
-                                 std::max(call.few.tiles, call.both ? call.many.tiles : 0), on));
+  return done(launch_paged_attention(call, static_cast<hipStream_t>(stream)));
 }
 
 }  // extern "C"

@@ -1,5 +1,4 @@
-// The 4-bit KV cache's format and arguments (kv4_cache.hip, paged_reserve.hip, paged_decode.hip,
-// paged_prefill.hip).
+// The 4-bit KV cache's format and arguments (kv4_cache.hip, paged_reserve.hip, paged_attention.hip).
 //
 // A key or value vector is held as blocks of 32 features: codes e2m1 (a sign and a magnitude of 0, 0.5, 1, 1.5, 2,
 // 3, 4 or 6, the even feature in a byte's low half) and an e8m0 scale byte s for 2^(s - 127), the operand format of
@@ -87,5 +86,22 @@ struct PagedArgs {
   float *part_o;  // [item][tile][D] unnormalised outputs of rows cut into runs
   float *part_ml;  // [item][tile][2] running maximum (log2 units) and sum
 };
+
+// A paged attention call: rows of few query vectors a KV head go to the decode kernel, the others, where the shapes
+// allow any, to the prefill kernel.
+struct PagedLaunch {
+  PagedArgs a;
+  int64_t items;  // blocks; 0: no launch
+  int tiles;      // of a row and KV head, at most
+  size_t bytes;   // records of rows cut into runs; 0: no row can be
+};
+struct PagedLaunches {
+  PagedLaunch few, many;
+  size_t bytes() const { return few.bytes + many.bytes; }
+};
+
+// Query vectors a KV head that one decode item takes at most (256 features leave registers for one group of 16).
+constexpr int paged_decode_columns(int dim) { return dim == 256 ? 16 : 32; }
+constexpr int kPagedPrefillTile = 128;  // query vectors of a prefill item
 
 }  // namespace xattn

@@ -2,6 +2,7 @@
 // (include/xinfer_attention.h), as torch_ops.cpp is over the other operators.  Outputs and workspaces come from the
 // caching allocator, launches go to the current stream of the inputs' device.
 #include <ATen/ATen.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/inductor/aoti_torch/utils.h>
@@ -19,22 +20,34 @@ namespace {
 
 using Tensors = std::initializer_list<const at::Tensor *>;
 
-xinfer_view4 view4(const at::Tensor &t) {
+// A view of `t` [B, H, T, D] or, with `token_major`, of `t` [B, T, H, D] as [B, H, T, D]: no tensor is made for it.
+xinfer_view4 view4(const at::Tensor &t, bool token_major = false) {
   xinfer_view4 v{};
   v.data = t.data_ptr();
+  const int order[4] = {0, token_major ? 2 : 1, token_major ? 1 : 2, 3};
   for (int i = 0; i < 4; ++i) {
-    v.size[i] = t.size(i);
-    v.stride[i] = t.stride(i);
+    v.size[i] = t.size(order[i]);
+    v.stride[i] = t.stride(order[i]);
   }
   return v;
+}
+// `t` [B, T, R] as [B, 1, T, R].
+xinfer_view4 view3(const at::Tensor &t) {
+  return xinfer_view4{t.data_ptr(), {t.size(0), 1, t.size(1), t.size(2)}, {t.stride(0), 0, t.stride(1), t.stride(2)}};
 }
 
 // Rows the kernels read in place: unit feature stride, other strides divisible by 8, 16-byte aligned data; others
 // are copied.
 at::Tensor in_rows(const at::Tensor &t) {
-  bool fine = (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) == 0 && (t.size(3) <= 1 || t.stride(3) == 1);
-  for (int i = 0; i < 3; ++i) fine = fine && (t.size(i) <= 1 || t.stride(i) % 8 == 0);
-  return fine ? t : t.contiguous(at::MemoryFormat::Contiguous);
+  const int64_t last = t.dim() - 1;
+  bool fine = (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) == 0 && (t.size(last) <= 1 || t.stride(last) == 1);
+  for (int64_t i = 0; i < last; ++i) fine = fine && (t.size(i) <= 1 || t.stride(i) % 8 == 0);
+  return fine ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+// A tensor on `like`'s device straight from the allocator (a call through the dispatcher takes twice the time).
+at::Tensor new_tensor(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor &like) {
+  return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt);
 }
 
 void *stream_of(const at::Tensor &t) {
@@ -94,9 +107,9 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> paged_kv_reserve(
   TORCH_CHECK(tokens >= 0, "Expected a number of new tokens");
   c10::DeviceGuard guard(kv_before.device());
   auto before = kv_before.contiguous(), after = kv_lengths.contiguous(), counts = query_lengths.contiguous();
-  auto lengths = at::empty({2, rows}, kv_before.options());
-  auto positions = at::empty({rows, tokens}, counters.options()), slots = at::empty({rows, tokens}, counters.options());
-  auto next = at::empty({2}, counters.options());
+  auto lengths = new_tensor({2, rows}, at::kInt, counters);
+  auto positions = new_tensor({rows, tokens}, at::kLong, counters), slots = new_tensor({rows, tokens}, at::kLong, counters);
+  auto next = new_tensor({2}, at::kLong, counters);
   auto ints = [](const at::Tensor &t) { return static_cast<int32_t *>(t.data_ptr()); };
   auto longs = [](const at::Tensor &t) { return static_cast<int64_t *>(t.data_ptr()); };
   check_status(xinfer_paged_kv_reserve(ints(before), ints(after), ints(counts), rows, tokens, page_size, longs(counters),
@@ -127,9 +140,8 @@ std::tuple<at::Tensor, at::Tensor> read_kv4(const at::Tensor &key_codes, const a
   TORCH_CHECK(slots.scalar_type() == at::kLong && slots.dim() == 2, "Expected int64 slots [B,T]");
   const auto cache = cache_of(key_codes, key_scales, value_codes, value_scales);
   c10::DeviceGuard guard(slots.device());
-  const auto options = slots.options().dtype(at::kBFloat16);
-  auto key = at::empty({slots.size(0), cache.kv_heads, slots.size(1), cache.dim}, options);
-  auto value = at::empty(key.sizes(), options);
+  auto key = new_tensor({slots.size(0), cache.kv_heads, slots.size(1), cache.dim}, at::kBFloat16, slots);
+  auto value = new_tensor(key.sizes(), at::kBFloat16, slots);
   check_status(xinfer_read_kv4(&cache, static_cast<const int64_t *>(slots.data_ptr()), slots.stride(0), slots.stride(1),
                                slots.size(0), slots.size(1), key.data_ptr(), value.data_ptr(), stream_of(slots)));
   return {key, value};
@@ -151,13 +163,11 @@ at::Tensor qk_norm_rope_append_kv4(const at::Tensor &q, const at::Tensor &key, c
   check_slots(slots, q.size(0), q.size(1));
   const auto cache = cache_of(key_codes, key_scales, value_codes, value_scales);
   c10::DeviceGuard guard(q.device());
-  auto output = at::empty({q.size(0), q.size(2), q.size(1), q.size(3)}, q.options());
+  auto output = new_tensor({q.size(0), q.size(2), q.size(1), q.size(3)}, at::kBFloat16, q);
+  const auto qr = in_rows(q), kr = in_rows(key), vr = in_rows(value), cr = in_rows(cos), sr = in_rows(sin);
+  const auto qw = in_rows(q_weight), kw = in_rows(k_weight);
   // Per-head views [B,H,T,D] and [B,1,T,R].
-  auto qh = in_rows(q.transpose(1, 2)), kh = in_rows(key.transpose(1, 2)), vh = in_rows(value.transpose(1, 2));
-  auto cs = in_rows(cos.unsqueeze(1)), sn = in_rows(sin.unsqueeze(1));
-  // in_rows of a rank-4 view: the weights as one row.
-  auto qw = in_rows(q_weight.view({1, 1, 1, -1})), kw = in_rows(k_weight.view({1, 1, 1, -1}));
-  auto qv = view4(qh), kv = view4(kh), vv = view4(vh), cv = view4(cs), sv = view4(sn);
+  const auto qv = view4(qr, true), kv = view4(kr, true), vv = view4(vr, true), cv = view3(cr), sv = view3(sr);
   check_status(xinfer_qk_norm_rope_append_kv4(&qv, &kv, &vv, qw.data_ptr(), kw.data_ptr(), eps, weight_offset, &cv, &sv,
                                               static_cast<const int64_t *>(slots.data_ptr()), slots.stride(0),
                                               slots.stride(1), output.data_ptr(), &cache, stream_of(q)));
@@ -180,14 +190,15 @@ at::Tensor paged_attention_kv4(const at::Tensor &q, const at::Tensor &key_codes,
   TORCH_CHECK(!q.requires_grad(), "xinfer attention supports inference only");
   const auto cache = cache_of(key_codes, key_scales, value_codes, value_scales);
   c10::DeviceGuard guard(q.device());
-  auto output = at::empty({q.size(0), q.size(2), q.size(1), q.size(3)}, q.options());
+  auto output = new_tensor({q.size(0), q.size(2), q.size(1), q.size(3)}, at::kBFloat16, q);
   auto query = in_rows(q);
   auto qv = view4(query);
   const size_t bytes = xinfer_paged_attention_kv4_workspace_size(&qv, &cache, block_table.size(1), max_length);
-  auto workspace = at::empty({static_cast<int64_t>(bytes)}, q.options().dtype(at::kByte));
+  at::Tensor workspace;
+  if (bytes > 0) workspace = new_tensor({static_cast<int64_t>(bytes)}, at::kByte, q);
   check_status(xinfer_paged_attention_kv4(&qv, &cache, static_cast<const int32_t *>(block_table.data_ptr()),
                                           block_table.size(1), static_cast<const int32_t *>(lengths.data_ptr()),
-                                          max_length, scale, output.data_ptr(), workspace.data_ptr(), bytes,
+                                          max_length, scale, output.data_ptr(), bytes > 0 ? workspace.data_ptr() : nullptr, bytes,
                                           stream_of(q)));
   return output;
 }

@@ -75,19 +75,11 @@ constexpr size_t kScratchBytes = size_t(32) << 20;
 // per device.
 hipError_t scratch_pointer(void **pointer);
 
-// The paged 4-bit KV cache (kv4_cache.hip, paged_reserve.hip, paged_decode.hip, paged_prefill.hip).
+// The paged 4-bit KV cache (kv4_cache.hip, paged_reserve.hip, paged_attention.hip).
 hipError_t launch_append_kv4(const Kv4AppendArgs &a, hipStream_t stream);
 hipError_t launch_read_kv4(const Kv4ReadArgs &a, hipStream_t stream);
 hipError_t launch_norm_rope_kv4(const Kv4NormRopeArgs &a, hipStream_t stream);
 hipError_t launch_reserve(const ReserveArgs &a, hipStream_t stream);
-// Query vectors a KV head that one item of the paged decode kernel takes at most (256 features leave registers for
-// one group of 16 columns).
-constexpr int paged_decode_columns(int dim) { return dim == 256 ? 16 : 32; }
-hipError_t launch_paged_decode(const PagedArgs &a, unsigned items, hipStream_t stream);
-// The paged prefill kernel: items of kPagedPrefillTile query vectors.
-constexpr int kPagedPrefillTile = 128;
-hipError_t launch_paged_prefill(const PagedArgs &a, unsigned items, hipStream_t stream);
-// Joins the runs of a decode launch and, if there is one, of a prefill launch; `tiles`: the most of a row and KV head.
-hipError_t launch_paged_merge(const PagedArgs &few, const PagedArgs *many, int tiles, hipStream_t stream);
+hipError_t launch_paged_attention(const PagedLaunches &l, hipStream_t stream);
 
 }  // namespace xattn

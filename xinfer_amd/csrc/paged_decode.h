@@ -1,6 +1,6 @@
 // Attention over the paged 4-bit cache for rows of few query vectors a KV head: single tokens and short runs of them.
 //
-// A block of 8 waves takes an item (paged_plan.h): up to 16 * NC query vectors of a (row, KV head) over a run of
+// A block takes an item (paged_plan.h): up to 16 * NC query vectors of a (row, KV head) over a run of
 // keys, one 64-key group at a time per wave.  A wave keeps the running maximum and sum of the softmax and its
 // output in registers; the waves meet in LDS at the end, runs in the merge kernel.
 //
@@ -13,13 +13,14 @@
 //
 // Weights are rounded to bf16.  With up to 8 vectors the other 8 columns hold what that rounding loses
 // (w - bf16(w)), at no further matrix work, which leaves 2^-17 of a weight; with more the rounding is up to 2^-9.
+#pragma once
+
 #include "paged_mfma.h"
 #include "paged_plan.h"
-#include "launch.h"
 
 namespace xattn {
 
-constexpr int kPagedWaves = 8, kPagedThreads = 64 * kPagedWaves;
+constexpr int kPagedWaves = 4;  // of a decode block
 constexpr float kLowest = -3.0e38f;  // running maximum before any key
 
 template <int D>
@@ -122,58 +123,96 @@ struct GroupLoads {
 template <int D>
 struct QueryOperand {
   using S = PagedShape<D>;
+  static constexpr int PIECES = D == 64 ? 1 : 2;
   u32x4 first[S::KC][2], second[S::KC][2];
   int scale[S::KC];
-  __device__ __forceinline__ void load(const uint16_t *q, bool there, int m, int g) {
+  // The column's features of this lane, zero where there is no such column.
+  __device__ __forceinline__ void fetch(const uint16_t *q, bool there, int g, u32x4 (&x)[S::KC][PIECES][2]) const {
+#pragma unroll
+    for (int c = 0; c < S::KC; ++c)
+#pragma unroll
+      for (int p = 0; p < PIECES; ++p)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) x[c][p][e] = there ? load16(q + 128 * c + 64 * p + 16 * g + 8 * e) : u32x4{0, 0, 0, 0};
+  }
+  __device__ __forceinline__ void convert(const u32x4 (&x)[S::KC][PIECES][2], int m, int g) {
 #pragma unroll
     for (int c = 0; c < S::KC; ++c) {
-      constexpr int PIECES = D == 64 ? 1 : 2;
-      uint32_t top[2] = {0, 0};
-      u32x4 x[2][2];
+      int s[2] = {127, 127};
 #pragma unroll
       for (int p = 0; p < PIECES; ++p) {
-        const uint16_t *const at = q + 128 * c + 64 * p + 16 * g;
-        x[p][0] = there ? load16(at) : u32x4{0, 0, 0, 0};
-        x[p][1] = there ? load16(at + 8) : u32x4{0, 0, 0, 0};
-        top[p] = largest(x[p][1], largest(x[p][0], 0u));
         // The block's other 16 features are in lane group g ^ 1.
-        const auto r = __builtin_amdgcn_permlane16_swap(top[p], top[p], false, false);
-        top[p] = max(r[0], r[1]);
+        const uint32_t top = largest(x[c][p][1], largest(x[c][p][0], 0u));
+        const auto r = __builtin_amdgcn_permlane16_swap(top, top, false, false);
+        s[p] = query_scale(max(r[0], r[1]));
+        split_query(x[c][p][0], x[c][p][1], s[p], first[c][p], second[c][p]);
       }
-      const int s0 = query_scale(top[0]), s1 = query_scale(top[1]);
-      split_query(x[0][0], x[0][1], s0, first[c][0], second[c][0]);
       if constexpr (D == 64) first[c][1] = second[c][1] = u32x4{0, 0, 0, 0};
-      else split_query(x[1][0], x[1][1], s1, first[c][1], second[c][1]);
       // Block g's scale is with lane group 2 (g % 2), of its first piece for g < 2.
-      const int from = m + 32 * (g & 1), b0 = __shfl(s0, from), b1 = __shfl(s1, from);
-      const int s = D == 64 || g < 2 ? b0 : b1;
-      scale[c] = s | (s == 255 ? 255 : s - 4) << 8;
+      const int from = m + 32 * (g & 1), b0 = __shfl(s[0], from), b1 = __shfl(s[1], from);
+      const int mine = D == 64 || g < 2 ? b0 : b1;
+      scale[c] = mine | (mine == 255 ? 255 : mine - 4) << 8;
     }
   }
 };
 
-template <int D, int NC>
-__global__ void __launch_bounds__(kPagedThreads, D == 256 || NC == 2 ? 2 : 4) paged_decode_kernel(const PagedArgs a) {
+// Scores of a group's keys against 16 queries: s[t][i] of lane (m, g) is query m's of key 16 g + 4 i + t.
+template <int D>
+__device__ __forceinline__ void paged_scores(const GroupLoads<D> &in, const QueryOperand<D> &q, int g, f32x4 (&s)[4]) {
   using S = PagedShape<D>;
-  constexpr int COLS = 16 * NC;
-  __shared__ __attribute__((aligned(1024))) char smem[kPagedWaves * S::STAGE];
-  __shared__ float2 wave_ml[kPagedWaves][16];
+  const f32x4 zero{0.0f, 0.0f, 0.0f, 0.0f};
+  if constexpr (D == 64) {
+    // Lane groups 0 and 1 hold tiles 0 and 1, lane groups 2 and 3 tiles 2 and 3, each half against zeros while the
+    // other counts; a scale beside a zero has to be finite.
+    const int low = g < 2 ? (int)in.ks[0] : 0x7f7f7f7f, high = g < 2 ? 0x7f7f7f7f : (int)in.ks[0];
+    const int ql = g < 2 ? q.scale[0] : 0x7f7f, qh = g < 2 ? 0x7f7f : q.scale[0];
+    const u32x4 none{0, 0, 0, 0};
+    const u32x4 f1[2] = {none, q.first[0][0]}, r1[2] = {none, q.second[0][0]};
+    s[0] = mfma16_fp4<0, 1>(in.k[0], q.second[0], mfma16_fp4<0, 0>(in.k[0], q.first[0], zero, low, ql), low, ql);
+    s[1] = mfma16_fp4<1, 1>(in.k[1], q.second[0], mfma16_fp4<1, 0>(in.k[1], q.first[0], zero, low, ql), low, ql);
+    s[2] = mfma16_fp4<2, 1>(in.k[0], r1, mfma16_fp4<2, 0>(in.k[0], f1, zero, high, qh), high, qh);
+    s[3] = mfma16_fp4<3, 1>(in.k[1], r1, mfma16_fp4<3, 0>(in.k[1], f1, zero, high, qh), high, qh);
+  } else {
+#pragma unroll
+    for (int t = 0; t < 4; ++t) s[t] = zero;
+#pragma unroll
+    for (int c = 0; c < S::KC; ++c) {
+      const int qs = q.scale[c], ks = (int)in.ks[c];
+      s[0] = mfma16_fp4<0, 1>(in.k[c], q.second[c], mfma16_fp4<0, 0>(in.k[c], q.first[c], s[0], ks, qs), ks, qs);
+      s[1] = mfma16_fp4<1, 1>(in.k[S::KC + c], q.second[c], mfma16_fp4<1, 0>(in.k[S::KC + c], q.first[c], s[1], ks, qs), ks, qs);
+      s[2] = mfma16_fp4<2, 1>(in.k[2 * S::KC + c], q.second[c], mfma16_fp4<2, 0>(in.k[2 * S::KC + c], q.first[c], s[2], ks, qs), ks, qs);
+      s[3] = mfma16_fp4<3, 1>(in.k[3 * S::KC + c], q.second[c], mfma16_fp4<3, 0>(in.k[3 * S::KC + c], q.first[c], s[3], ks, qs), ks, qs);
+    }
+  }
+}
+
+// LDS of a decode block: the waves' staged values (then outputs), their maxima and sums.
+template <int D, int WAVES>
+constexpr int kPagedDecodeLds = WAVES * (PagedShape<D>::STAGE + 16 * 8);
+
+// Item `index` of the plan, by the whole block; smem: kPagedDecodeLds bytes, 1024-byte aligned.
+template <int D, int NC, int WAVES>
+__device__ __forceinline__ void paged_decode_item(const PagedArgs &a, int index, char *smem) {
+  using S = PagedShape<D>;
+  constexpr int COLS = 16 * NC, THREADS = 64 * WAVES;
+  f32x2 *const wave_ml = reinterpret_cast<f32x2 *>(smem + WAVES * S::STAGE);
   const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   PagedItem it;
-  if (!paged_item(a, blockIdx.x, it)) return;
-  if (it.count < a.T) paged_zero_padded<D, kPagedThreads>(a, it);
+  if (!paged_item(a, index, it)) return;
+  if (it.count < a.T) paged_zero_padded<D, THREADS>(a, it);
   if (it.count == 0) return;
   const int vectors = min(it.count * a.G - it.tile * COLS, COLS);
   const bool twice = NC == 1 && vectors <= 8;  // columns 8..15 repeat the queries and take the weights' rests
 
   QueryOperand<D> q[NC];
+  u32x4 qx[NC][S::KC][QueryOperand<D>::PIECES][2];
   int last_key[NC];  // the last key that this lane's query sees
 #pragma unroll
   for (int n = 0; n < NC; ++n) {
     const int column = twice ? m & 7 : m + 16 * n, j = it.tile * COLS + column, t = j / a.G;
     const bool there = column < vectors;
-    q[n].load(a.q.p + it.row * a.q.sb + (it.h * a.G + (j - t * a.G)) * a.q.sh + t * a.q.st, there, m, g);
+    q[n].fetch(a.q.p + it.row * a.q.sb + (it.h * a.G + (j - t * a.G)) * a.q.sh + t * a.q.st, there, g, qx[n]);
     last_key[n] = there ? it.length - it.count + t : -1;
   }
   const int all_see = it.length - it.count + it.tile * COLS / a.G;  // every query sees keys up to this one
@@ -203,44 +242,19 @@ __global__ void __launch_bounds__(kPagedThreads, D == 256 || NC == 2 ? 2 : 4) pa
   // would have the compiler keep two groups in registers.
   GroupLoads<D> in;
   in.init(1 << a.cache.page_shift, (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)stage, m, g);
-  int group = it.group_begin + wave, page = page_of(group), next_page = page_of(group + kPagedWaves);
+  int group = it.group_begin + wave, page = page_of(group), next_page = page_of(group + WAVES);
   if (group < it.group_end) {
     in.keys(a, max(page, 0), it.h, place(group));
     in.values(a, max(page, 0), it.h, place(group));
   }
-  for (; group < it.group_end; group += kPagedWaves) {
+#pragma unroll
+  for (int n = 0; n < NC; ++n) q[n].convert(qx[n], m, g);
+  for (; group < it.group_end; group += WAVES) {
     in.renew();
-    const int next = group + kPagedWaves, after_page = page_of(next + kPagedWaves), load_page = max(next_page, 0);
+    const int next = group + WAVES, after_page = page_of(next + WAVES), load_page = max(next_page, 0);
     f32x4 s[NC][4];
-    const f32x4 zero{0.0f, 0.0f, 0.0f, 0.0f};
-    // A scale beside a zero operand (D = 64: one half of the lanes) has to be finite.
-    const int low = D == 64 ? (g < 2 ? (int)in.ks[0] : 0x7f7f7f7f) : 0, high = D == 64 ? (g < 2 ? 0x7f7f7f7f : (int)in.ks[0]) : 0;
 #pragma unroll
-    for (int n = 0; n < NC; ++n) {
-      if constexpr (D == 64) {
-        const u32x4 none{0, 0, 0, 0};
-        const u32x4 f1[2] = {none, q[n].first[0][0]}, r1[2] = {none, q[n].second[0][0]};
-        const int ql = g < 2 ? q[n].scale[0] : 0x7f7f, qh = g < 2 ? 0x7f7f : q[n].scale[0];
-        s[n][0] = mfma16_fp4<0, 1>(in.k[0], q[n].second[0], mfma16_fp4<0, 0>(in.k[0], q[n].first[0], zero, low, ql), low, ql);
-        s[n][1] = mfma16_fp4<1, 1>(in.k[1], q[n].second[0], mfma16_fp4<1, 0>(in.k[1], q[n].first[0], zero, low, ql), low, ql);
-        s[n][2] = mfma16_fp4<2, 1>(in.k[0], r1, mfma16_fp4<2, 0>(in.k[0], f1, zero, high, qh), high, qh);
-        s[n][3] = mfma16_fp4<3, 1>(in.k[1], r1, mfma16_fp4<3, 0>(in.k[1], f1, zero, high, qh), high, qh);
-      } else {
-#pragma unroll
-        for (int t = 0; t < 4; ++t) s[n][t] = zero;
-#pragma unroll
-        for (int c = 0; c < S::KC; ++c) {
-          const int qs = q[n].scale[c], ks = (int)in.ks[c];
-          s[n][0] = mfma16_fp4<0, 1>(in.k[c], q[n].second[c], mfma16_fp4<0, 0>(in.k[c], q[n].first[c], s[n][0], ks, qs), ks, qs);
-          s[n][1] = mfma16_fp4<1, 1>(in.k[S::KC + c], q[n].second[c],
-                                     mfma16_fp4<1, 0>(in.k[S::KC + c], q[n].first[c], s[n][1], ks, qs), ks, qs);
-          s[n][2] = mfma16_fp4<2, 1>(in.k[2 * S::KC + c], q[n].second[c],
-                                     mfma16_fp4<2, 0>(in.k[2 * S::KC + c], q[n].first[c], s[n][2], ks, qs), ks, qs);
-          s[n][3] = mfma16_fp4<3, 1>(in.k[3 * S::KC + c], q[n].second[c],
-                                     mfma16_fp4<3, 0>(in.k[3 * S::KC + c], q[n].first[c], s[n][3], ks, qs), ks, qs);
-        }
-      }
-    }
+    for (int n = 0; n < NC; ++n) paged_scores<D>(in, q[n], g, s[n]);
     // The scores are taken here, before the registers of their keys are loaded anew.
 #pragma unroll
     for (int n = 0; n < NC; ++n) asm volatile("" : "+v"(s[n][0]), "+v"(s[n][1]), "+v"(s[n][2]), "+v"(s[n][3]) : : "memory");
@@ -317,28 +331,28 @@ __global__ void __launch_bounds__(kPagedThreads, D == 256 || NC == 2 ? 2 : 4) pa
     }
     __syncthreads();
     const int columns = min(vectors - 16 * n, 16);
-    if (g == 0) wave_ml[wave][m] = float2{top[n], l};
+    if (g == 0) wave_ml[16 * wave + m] = f32x2{top[n], l};
     if (m < columns) {
 #pragma unroll
       for (int d = 0; d < S::DT; ++d)
         *reinterpret_cast<f32x4 *>(stage + m * (4 * D) + ((4 * d + g) ^ (m & 7)) * 16) = o[n][d];
     }
     __syncthreads();
-    for (int i = tid; i < columns * (D / 4); i += kPagedThreads) {
+    for (int i = tid; i < columns * (D / 4); i += THREADS) {
       const int column = i / (D / 4), f = i - column * (D / 4);
       float best = kLowest, total = 0.0f;
 #pragma unroll
-      for (int w = 0; w < kPagedWaves; ++w) best = fmaxf(best, wave_ml[w][column].x);
+      for (int w = 0; w < WAVES; ++w) best = fmaxf(best, wave_ml[16 * w + column].x);
       f32x4 out{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int w = 0; w < kPagedWaves; ++w) {
-        const float2 ml = wave_ml[w][column];
+      for (int w = 0; w < WAVES; ++w) {
+        const f32x2 ml = wave_ml[16 * w + column];
         const float keep = fast_exp2(ml.x - best);
         total += ml.y * keep;
         out += *reinterpret_cast<const f32x4 *>(smem + w * S::STAGE + column * (4 * D) + (f ^ (column & 7)) * 16) * keep;
       }
       if (it.nsplit > 1) {
-        const int64_t record = (int64_t)blockIdx.x * COLS + 16 * n + column;
+        const int64_t record = (int64_t)index * COLS + 16 * n + column;
         *as_global(reinterpret_cast<f32x4 *>(a.part_o + record * D + 4 * f)) = out;
         if (f == 0) *as_global(reinterpret_cast<f32x2 *>(a.part_ml + 2 * record)) = f32x2{best, total};
       } else {
@@ -351,65 +365,6 @@ __global__ void __launch_bounds__(kPagedThreads, D == 256 || NC == 2 ? 2 : 4) pa
       }
     }
   }
-}
-
-// Joins the runs of a (row, KV head, tile) of either launch (blockIdx.z).
-template <int D>
-__global__ void __launch_bounds__(256) paged_merge_kernel(const PagedArgs few, const PagedArgs many) {
-  const PagedArgs &a = blockIdx.z == 0 ? few : many;
-  const int tile = blockIdx.x / a.cache.Hkv, h = blockIdx.x - tile * a.cache.Hkv;
-  PagedItem it;
-  paged_row_items(a, blockIdx.y, it);
-  if (it.nsplit <= 1 || tile >= it.tiles) return;
-  const int vectors = min(it.count * a.G - tile * a.tile, a.tile);
-  for (int i = threadIdx.x; i < vectors * (D / 4); i += 256) {
-    const int column = i / (D / 4), f = i - column * (D / 4);
-    float best = kLowest, total = 0.0f;
-    f32x4 out{0.0f, 0.0f, 0.0f, 0.0f};
-    for (int s = 0; s < it.nsplit; ++s) {
-      const int64_t record = ((int64_t)it.begin + (int64_t)(tile * it.nsplit + s) * a.cache.Hkv + h) * a.tile + column;
-      const f32x2 ml = *as_global(reinterpret_cast<const f32x2 *>(a.part_ml + 2 * record));
-      const f32x4 part = *as_global(reinterpret_cast<const f32x4 *>(a.part_o + record * D + 4 * f));
-      const float now = fmaxf(best, ml.x), old = fast_exp2(best - now), keep = fast_exp2(ml.x - now);
-      best = now;
-      total = total * old + ml.y * keep;
-      out = out * old + part * keep;
-    }
-    const int j = tile * a.tile + column, t = j / a.G;
-    const float by = total == 0.0f ? 0.0f : 1.0f / total;
-    out *= by;
-    *as_global(reinterpret_cast<u32x2 *>(
-        a.out + (((int64_t)it.row * a.T + t) * a.Hq + h * a.G + (j - t * a.G)) * D + 4 * f)) =
-        u32x2{pack_bf16x2(out[0], out[1]), pack_bf16x2(out[2], out[3])};
-  }
-}
-
-template <int D>
-static void launch_decode_d(const PagedArgs &a, unsigned items, hipStream_t stream) {
-  if constexpr (paged_decode_columns(D) == 32) {
-    if (a.tile == 32) hipLaunchKernelGGL((paged_decode_kernel<D, 2>), dim3(items), dim3(kPagedThreads), 0, stream, a);
-  }
-  if (a.tile == 16) hipLaunchKernelGGL((paged_decode_kernel<D, 1>), dim3(items), dim3(kPagedThreads), 0, stream, a);
-}
-
-hipError_t launch_paged_decode(const PagedArgs &a, unsigned items, hipStream_t stream) {
-  switch (a.cache.D) {
-    case 64: launch_decode_d<64>(a, items, stream); break;
-    case 128: launch_decode_d<128>(a, items, stream); break;
-    default: launch_decode_d<256>(a, items, stream); break;
-  }
-  return hipGetLastError();
-}
-
-hipError_t launch_paged_merge(const PagedArgs &few, const PagedArgs *many, int tiles, hipStream_t stream) {
-  const dim3 grid(tiles * few.cache.Hkv, few.B, many ? 2 : 1);
-  const PagedArgs &other = many ? *many : few;
-  switch (few.cache.D) {
-    case 64: hipLaunchKernelGGL((paged_merge_kernel<64>), grid, dim3(256), 0, stream, few, other); break;
-    case 128: hipLaunchKernelGGL((paged_merge_kernel<128>), grid, dim3(256), 0, stream, few, other); break;
-    default: hipLaunchKernelGGL((paged_merge_kernel<256>), grid, dim3(256), 0, stream, few, other); break;
-  }
-  return hipGetLastError();
 }
 
 }  // namespace xattn

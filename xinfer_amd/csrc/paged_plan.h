@@ -47,76 +47,87 @@ __device__ __forceinline__ PagedShare paged_share(const PagedArgs &a, const Page
   return s;
 }
 
+// Rows 64 at a time, one a lane: what the plan looks at.  The first 64 stay in registers.
+struct PagedRows {
+  PagedRow p;
+  PagedShare s;
+  __device__ __forceinline__ void load(const PagedArgs &a, int base) {
+    const int r = base + (int)(threadIdx.x & 63);
+    p = PagedRow{0, 0};
+    s = PagedShare{0, 0};
+    if (r < a.B) {
+      p = paged_row(a, r);
+      s = paged_share(a, p);
+    }
+  }
+};
+
 // Groups of a run at most.
-__device__ __forceinline__ int paged_run(const PagedArgs &a) {
-  const int lane = threadIdx.x & 63;
-  float total = 0.0f;
-  for (int base = 0; base < a.B; base += 64) {
-    PagedShare s{0, 0};
-    if (base + lane < a.B) s = paged_share(a, paged_row(a, base + lane));
-    total += (float)s.groups * (float)s.tiles;
+__device__ __forceinline__ int paged_run(const PagedArgs &a, const PagedRows &first) {
+  float total = (float)first.s.groups * (float)first.s.tiles;
+  for (int base = 64; base < a.B; base += 64) {
+    PagedRows rows;
+    rows.load(a, base);
+    total += (float)rows.s.groups * (float)rows.s.tiles;
   }
   total = group_sum<64>(total) * (float)a.cache.Hkv;
   return max(a.min_groups, (int)(total / (float)a.target) + 1);
 }
 __device__ __forceinline__ int paged_splits(const PagedShare &s, int run) { return max(1, (s.groups + run - 1) / run); }
 
+// What lane `at` holds of its row; upto: items up to and with it.
+__device__ __forceinline__ void paged_take(PagedItem &it, const PagedRows &rows, int nsplit, int upto, int items, int at) {
+  it.count = __builtin_amdgcn_readlane(rows.p.count, at);
+  it.length = __builtin_amdgcn_readlane(rows.p.length, at);
+  it.nsplit = __builtin_amdgcn_readlane(nsplit, at);
+  it.tiles = __builtin_amdgcn_readlane(rows.s.tiles, at);
+  it.begin = __builtin_amdgcn_readlane(upto - items, at);
+  it.group_end = __builtin_amdgcn_readlane(rows.s.groups, at);
+}
+
 // Item `index` of the plan; false past its last.  Every lane of a wave calls it, with the same index.
 __device__ __forceinline__ bool paged_item(const PagedArgs &a, int index, PagedItem &it) {
-  const int lane = threadIdx.x & 63, run = paged_run(a), Hkv = a.cache.Hkv;
-  int before = 0;
-  for (int base = 0; base < a.B; base += 64) {
-    PagedRow p{0, 0};
-    PagedShare s{0, 0};
-    if (base + lane < a.B) {
-      p = paged_row(a, base + lane);
-      s = paged_share(a, p);
-    }
-    const int nsplit = paged_splits(s, run), items = s.tiles * nsplit * Hkv, upto = before + wave_scan(items);
+  const int Hkv = a.cache.Hkv;
+  PagedRows rows;
+  rows.load(a, 0);
+  const int run = paged_run(a, rows);
+  for (int base = 0, before = 0;;) {
+    const int nsplit = paged_splits(rows.s, run), items = rows.s.tiles * nsplit * Hkv, upto = before + wave_scan(items);
     const uint64_t past = __ballot(upto > index);
     if (past != 0) {
       const int at = __builtin_ctzll(past);
       it.row = base + at;
-      it.count = __builtin_amdgcn_readlane(p.count, at);
-      it.length = __builtin_amdgcn_readlane(p.length, at);
-      it.nsplit = __builtin_amdgcn_readlane(nsplit, at);
-      it.tiles = __builtin_amdgcn_readlane(s.tiles, at);
-      it.begin = __builtin_amdgcn_readlane(upto - items, at);
-      const int groups = __builtin_amdgcn_readlane(s.groups, at);
-      const int i = index - it.begin, rest = i / Hkv;
+      paged_take(it, rows, nsplit, upto, items, at);
+      const uint32_t i = index - it.begin, rest = i / (uint32_t)Hkv;
       it.h = i - rest * Hkv;
-      it.tile = rest / it.nsplit;
+      it.tile = rest / (uint32_t)it.nsplit;
       it.split = rest - it.tile * it.nsplit;
-      it.group_begin = (int)((int64_t)groups * it.split / it.nsplit);
-      it.group_end = (int)((int64_t)groups * (it.split + 1) / it.nsplit);
+      // The first `more` runs take one group more than the others.
+      const int groups = it.group_end, each = (uint32_t)groups / (uint32_t)it.nsplit, more = groups - each * it.nsplit;
+      it.group_begin = it.split * each + min(it.split, more);
+      it.group_end = it.group_begin + each + (it.split < more ? 1 : 0);
       return true;
     }
+    base += 64;
+    if (base >= a.B) return false;
     before = __builtin_amdgcn_readlane(upto, 63);
+    rows.load(a, base);
   }
-  return false;
 }
 
 // Row `row`'s part of the plan: its first item, splits and tiles.
 __device__ __forceinline__ void paged_row_items(const PagedArgs &a, int row, PagedItem &it) {
-  const int lane = threadIdx.x & 63, run = paged_run(a), Hkv = a.cache.Hkv;
-  int before = 0;
-  for (int base = 0; base <= row; base += 64) {
-    PagedRow p{0, 0};
-    PagedShare s{0, 0};
-    if (base + lane < a.B) {
-      p = paged_row(a, base + lane);
-      s = paged_share(a, p);
-    }
-    const int nsplit = paged_splits(s, run), items = s.tiles * nsplit * Hkv, upto = before + wave_scan(items);
+  PagedRows rows;
+  rows.load(a, 0);
+  const int run = paged_run(a, rows);
+  for (int base = 0, before = 0;; rows.load(a, base)) {
+    const int nsplit = paged_splits(rows.s, run), items = rows.s.tiles * nsplit * a.cache.Hkv, upto = before + wave_scan(items);
     if (row < base + 64) {
-      const int at = row - base;
       it.row = row;
-      it.count = __builtin_amdgcn_readlane(p.count, at);
-      it.length = __builtin_amdgcn_readlane(p.length, at);
-      it.nsplit = __builtin_amdgcn_readlane(nsplit, at);
-      it.tiles = __builtin_amdgcn_readlane(s.tiles, at);
-      it.begin = __builtin_amdgcn_readlane(upto - items, at);
+      paged_take(it, rows, nsplit, upto, items, row - base);
+      return;
     }
+    base += 64;
     before = __builtin_amdgcn_readlane(upto, 63);
   }
 }

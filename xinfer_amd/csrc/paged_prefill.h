@@ -1,7 +1,7 @@
 // Attention over the paged 4-bit cache for rows of many query vectors a KV head: prompt chunks.
 //
-// A block of 4 waves takes an item (paged_plan.h): 128 query vectors of a (row, KV head), 32 a wave, over a run of
-// keys in 64-key groups.  A wave reads the group's keys as they lie in the cache, as the A operand of the scaled
+// A block takes an item (paged_plan.h): 128 query vectors of a (row, KV head) over a run of keys in 64-key groups.  Up
+// to 128 features it has 4 waves of 32 vectors each (paged_chunk_item).  A wave reads the group's keys as they lie in the cache, as the A operand of the scaled
 // 32x32x64 product against its queries' two e4m3 terms (paged_mfma.h): row m of tile t (of two) is key 2 m + t, so a
 // lane's two keys have their scales in neighbouring bytes.  A lane (column q, half h) then holds 32 scores of its query,
 // and for each 16 keys 8 neighbouring ones, which is the B operand of the bf16 PV product: nothing of the softmax
@@ -10,15 +10,21 @@
 // The block turns the group's values into bf16 (exact) in LDS together, one group ahead, and every wave reads
 // them transposed as the A operand.  One barrier a group.
 //
+// 256 features of 32 vectors would take 128 registers for the output and 64 for the queries, which leaves no two
+// waves a SIMD.  There 8 waves take 16 vectors each (paged_chunk_item_wide), with the products and layouts of the
+// decode kernel (paged_decode.h) but values staged by the whole block.
+//
 // Weights are rounded to bf16 (2^-9 of a weight at most, on average lost in the sum); their sum is taken before.
-#include "paged_mfma.h"
-#include "paged_plan.h"
-#include "launch.h"
+#pragma once
+
+#include "paged_decode.h"
 
 namespace xattn {
 
 constexpr int kChunkWaves = 4, kChunkThreads = 64 * kChunkWaves;
-constexpr float kLowestMax = -3.0e38f;  // running maximum before any key
+constexpr int kWideWaves = 8;
+// Waves of a prefill block.
+constexpr int paged_chunk_waves(int dim) { return dim == 256 ? kWideWaves : kChunkWaves; }
 
 template <int D>
 struct ChunkShape {
@@ -36,20 +42,19 @@ __device__ __forceinline__ int chunk_swizzle(int r) {
   return D == 64 ? 5 * ((r >> 1) & 1) : 5 * (r & 3);
 }
 
-typedef short i16x4p __attribute__((ext_vector_type(4)));
-__device__ __forceinline__ u32x2 lds_transposed(uint32_t lds) {
-  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4p *)(lds)));
-}
-
+// LDS of a prefill block: staged groups.
 template <int D>
-__global__ void __launch_bounds__(kChunkThreads, D == 256 ? 1 : 2) paged_prefill_kernel(const PagedArgs a) {
+constexpr int kPagedChunkLds = (D == 256 ? 3 : 2) * 64 * 2 * D;
+
+// Item `index` of the plan, by the whole block; smem: kPagedChunkLds bytes, 1024-byte aligned.
+template <int D>
+__device__ __forceinline__ void paged_chunk_item(const PagedArgs &a, int index, char *smem) {
   using S = ChunkShape<D>;
   constexpr int COLS = 32 * kChunkWaves;
-  __shared__ __attribute__((aligned(1024))) char smem[2 * S::STAGE];
   const int tid = threadIdx.x, lane = tid & 63, m = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   PagedItem it;
-  if (!paged_item(a, blockIdx.x, it)) return;
+  if (!paged_item(a, index, it)) return;
   paged_zero_padded<D, kChunkThreads>(a, it);
 
   // This wave's queries.
@@ -90,7 +95,7 @@ __global__ void __launch_bounds__(kChunkThreads, D == 256 ? 1 : 2) paged_prefill
   for (int d = 0; d < S::DT; ++d)
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[d][r] = 0.0f;
-  float top = kLowestMax, sum = 0.0f;
+  float top = kLowest, sum = 0.0f;
 
   const int shift = a.cache.page_shift - 6, size = 1 << a.cache.page_shift;
   typedef const __attribute__((address_space(4))) int32_t *table_ptr;
@@ -218,7 +223,7 @@ __global__ void __launch_bounds__(kChunkThreads, D == 256 ? 1 : 2) paged_prefill
 #pragma unroll
         for (int d = 0; d < S::DT; ++d) {
           const uint32_t at = (get ^ (64 * d) ^ (d >= 4 ? 16 : 0)) + 16 * b * S::ROW;
-          const u32x2 lo = lds_transposed(at), hi = lds_transposed(at + 4 * S::ROW);
+          const u32x2 lo = read_transposed(at), hi = read_transposed(at + 4 * S::ROW);
           o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(u32x4{lo.x, lo.y, hi.x, hi.y}), weights, o[d], 0, 0, 0);
         }
       }
@@ -229,7 +234,7 @@ __global__ void __launch_bounds__(kChunkThreads, D == 256 ? 1 : 2) paged_prefill
   if (!there) return;
   // o[d][r] is feature 32 d + 8 (r / 4) + 4 h + r % 4.
   if (it.nsplit > 1) {
-    const int64_t record = (int64_t)blockIdx.x * COLS + 32 * wave + m;
+    const int64_t record = (int64_t)index * COLS + 32 * wave + m;
 #pragma unroll
     for (int d = 0; d < S::DT; ++d)
 #pragma unroll
@@ -249,13 +254,174 @@ __global__ void __launch_bounds__(kChunkThreads, D == 256 ? 1 : 2) paged_prefill
   }
 }
 
-hipError_t launch_paged_prefill(const PagedArgs &a, unsigned items, hipStream_t stream) {
-  switch (a.cache.D) {
-    case 64: hipLaunchKernelGGL((paged_prefill_kernel<64>), dim3(items), dim3(kChunkThreads), 0, stream, a); break;
-    case 128: hipLaunchKernelGGL((paged_prefill_kernel<128>), dim3(items), dim3(kChunkThreads), 0, stream, a); break;
-    default: hipLaunchKernelGGL((paged_prefill_kernel<256>), dim3(items), dim3(kChunkThreads), 0, stream, a); break;
+// The same for 256 features: 8 waves of 16 query vectors.
+template <int D>
+__device__ __forceinline__ void paged_chunk_item_wide(const PagedArgs &a, int index, char *smem) {
+  using S = PagedShape<D>;
+  constexpr int WAVES = kWideWaves, THREADS = 64 * WAVES, COLS = 16 * WAVES, BLOCKS = D / 32, STAGE = 64 * S::ROW;
+  static_assert(64 * BLOCKS == THREADS, "a thread stages one block of one key");
+  const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  PagedItem it;
+  if (!paged_item(a, index, it)) return;
+  paged_zero_padded<D, THREADS>(a, it);
+
+  const int vectors = it.count * a.G, wave_first = it.tile * COLS + 16 * wave, j = wave_first + m;
+  const int t = j / a.G, head = it.h * a.G + (j - t * a.G);
+  const bool there = j < vectors;
+  const int last_key = there ? it.length - it.count + t : -1;
+  const int all_see = it.length - it.count + wave_first / a.G;  // all of the wave's queries see keys up to this one,
+  const int none_see = wave_first < vectors                     // and none of them this one or a later
+                           ? it.length - it.count + (min(wave_first + 16, vectors) - 1) / a.G + 1 : 0;
+  const int tile_end = it.length - it.count + (min(it.tile * COLS + COLS, vectors) - 1) / a.G + 1;
+  const int group_end = min(it.group_end, (tile_end + kGroupKeys - 1) / kGroupKeys);
+  QueryOperand<D> q;
+  u32x4 qx[S::KC][QueryOperand<D>::PIECES][2];
+  q.fetch(a.q.p + it.row * a.q.sb + head * a.q.sh + t * a.q.st, there, g, qx);
+
+  f32x4 o[S::DT];
+#pragma unroll
+  for (int d = 0; d < S::DT; ++d) o[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  float top = kLowest, sum = 0.0f;
+
+  const int shift = a.cache.page_shift - 6, size = 1 << a.cache.page_shift;
+  typedef const __attribute__((address_space(4))) int32_t *table_ptr;
+  const table_ptr table = (table_ptr)(a.table + (int64_t)it.row * a.width);
+  auto page_of = [&](int group) {
+    const int page = group < group_end ? table[group >> shift] : -1;
+    return page >= 0 && page < a.cache.pages ? page : -1;
+  };
+  auto place = [&](int group) { return (group & ((1 << shift) - 1)) * kGroupKeys; };
+
+  // Staged values: 16-byte chunk c of key r lies at slot c ^ S(r) ^ (c / 16), which spreads over the banks the eight
+  // blocks of a key that eight lanes store, and the 16 rows of a transposing read.
+  auto swizzle = [](int r) { return 2 * ((r & 3) + 4 * ((r >> 4) & 1)); };
+  const int key = tid / BLOCKS, block = tid % BLOCKS;
+  const uint32_t stage = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)smem;
+  const uint32_t put_at = stage + key * S::ROW + ((4 * block) ^ swizzle(key) ^ (block >> 2)) * 16;
+  const int x = 16 * g + (m >> 2);
+  uint32_t get_at = stage + x * S::ROW + (((m & 3) >> 1) ^ swizzle(x)) * 16 + 8 * (m & 1);
+  u32x4 v;
+  uint32_t vs;
+  auto load_values = [&](int group, int page) {
+    const int64_t hd = (int64_t)max(page, 0) * a.cache.Hkv + it.h;
+    v = *as_global(reinterpret_cast<const u32x4 *>(a.cache.value + (hd * size + place(group)) * (D / 2) + 16 * tid));
+    vs = *as_global(a.cache.value_scale + hd * BLOCKS * size + place(group) + (uint32_t)(block * size + key));
+  };
+  auto put_values = [&](int buffer) {
+    const float scale = kv4_scale_value(min((int)vs, kKv4MaxScale));
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      *(__attribute__((address_space(3))) u32x4 *)((put_at ^ (16 * c)) + buffer * STAGE) = kv4_values(v[c], scale);
+  };
+
+  GroupLoads<D> in;
+  in.init(size, stage, m, g);
+  f32x4 s[4];
+  uint32_t pw[2][4];
+  // A group's scores, then the loads of the next one's keys.
+  auto scores = [&](int next, int next_page) {
+    paged_scores<D>(in, q, g, s);
+    asm volatile("" : "+v"(s[0]), "+v"(s[1]), "+v"(s[2]), "+v"(s[3]) : : "memory");
+    in.keys(a, max(next_page, 0), it.h, place(next));
+  };
+  // Weights of a group: s[t][i] is key 16 g + 4 i + t.
+  auto weights = [&](int group, int page) {
+    if (group * kGroupKeys + kGroupKeys - 1 > all_see || page < 0) {
+      const int at = group * kGroupKeys + 16 * g, last = page < 0 ? -1 : last_key;
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[u][i] = at + 4 * i + u <= last ? s[u][i] : -INFINITY;
+    }
+    float best = fmaxf(fmaxf(s[0][0], s[1][0]), fmaxf(s[2][0], s[3][0]));
+#pragma unroll
+    for (int i = 1; i < 4; ++i) best = fmaxf(best, fmaxf(fmaxf(s[0][i], s[1][i]), fmaxf(s[2][i], s[3][i])));
+    best = fmaxf(top, pair_max32(pair_max16(best)) * a.scale_log2);
+    if (__any(best > top)) {
+      const float keep = fast_exp2(top - best);
+      sum *= keep;
+#pragma unroll
+      for (int d = 0; d < S::DT; ++d) o[d] *= keep;
+      top = best;
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const int i = 2 * u + w / 2, z = 2 * (w & 1);
+        const float p0 = fast_exp2(fmaf(s[z][i], a.scale_log2, -top)), p1 = fast_exp2(fmaf(s[z + 1][i], a.scale_log2, -top));
+        sum += p0 + p1;
+        pw[u][w] = pack_bf16x2(p0, p1);
+      }
+  };
+  auto output = [&](int buffer) {
+    const uint32_t get = get_at + buffer * STAGE;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const bf16x8 w = as_bf16x8(u32x4{pw[u][0], pw[u][1], pw[u][2], pw[u][3]});
+#pragma unroll
+      for (int d = 0; d < S::DT; ++d) {
+        const uint32_t at = (get ^ (32 * d) ^ (d >= 8 ? 16 : 0)) + 8 * u * S::ROW;
+        const u32x2 lo = read_transposed(at), hi = read_transposed(at + 4 * S::ROW);
+        o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(u32x4{lo.x, lo.y, hi.x, hi.y}), w, o[d], 0, 0, 0);
+      }
+    }
+  };
+  // Waves w and w + 4 share a SIMD.  Between two barriers the first half of the waves computes weights, then the
+  // matrix products (this group's output, the next one's scores); the second half the products first (the last
+  // group's output, this one's scores), then weights: one's matrix work runs beside the other's vector work.  So three
+  // groups' values are staged: the last, this and the next one.
+  const bool ahead = wave < WAVES / 2;
+  const int begin = it.group_begin;
+  if (begin < group_end) {
+    int page = page_of(begin), next_page = page_of(begin + 1);
+    load_values(begin, page);
+    in.keys(a, max(page, 0), it.h, place(begin));
+    q.convert(qx, m, g);
+    put_values(0);
+    load_values(begin + 1, next_page);
+    if (ahead) scores(begin + 1, next_page);
+    int last = 2, now = 0, next = 1;  // staged groups' buffers
+    for (int group = begin; group < group_end; ++group) {
+      asm volatile("" : "+v"(in.key_at), "+v"(in.key_scale_at), "+v"(get_at));
+      const int after_page = page_of(group + 2);
+      const bool active = group * kGroupKeys < none_see;  // uniform in the wave
+      __syncthreads();  // every wave has stored its part of this group's values
+      if (!ahead) {
+        if (group > begin && (group - 1) * kGroupKeys < none_see) output(last);
+        scores(group + 1, next_page);
+      }
+      put_values(next);
+      load_values(group + 2, after_page);
+      if (active) weights(group, page);
+      if (ahead) {
+        if (active) output(now);
+        scores(group + 2, after_page);
+      }
+      page = next_page, next_page = after_page;
+      const int free = last;
+      last = now, now = next, next = free;
+    }
+    if (!ahead && (group_end - 1) * kGroupKeys < none_see) output(last);
   }
-  return hipGetLastError();
+
+  sum = pair_sum32(pair_sum16(sum));
+  if (!there) return;
+  // o[d][i] is feature 16 d + 4 g + i.
+  if (it.nsplit > 1) {
+    const int64_t record = (int64_t)index * COLS + 16 * wave + m;
+#pragma unroll
+    for (int d = 0; d < S::DT; ++d) *as_global(reinterpret_cast<f32x4 *>(a.part_o + record * D + 16 * d + 4 * g)) = o[d];
+    if (g == 0) *as_global(reinterpret_cast<f32x2 *>(a.part_ml + 2 * record)) = f32x2{top, sum};
+  } else {
+    const float by = sum == 0.0f ? 0.0f : 1.0f / sum;
+    uint16_t *const out = a.out + (((int64_t)it.row * a.T + t) * a.Hq + head) * D + 4 * g;
+#pragma unroll
+    for (int d = 0; d < S::DT; ++d)
+      *as_global(reinterpret_cast<u32x2 *>(out + 16 * d)) =
+          u32x2{pack_bf16x2(o[d][0] * by, o[d][1] * by), pack_bf16x2(o[d][2] * by, o[d][3] * by)};
+  }
 }
 
 }  // namespace xattn

@@ -24,12 +24,19 @@ PAGE_SIZES = (64, 128, 256)
 HEAD_DIMS = (64, 128, 256)
 
 
-def _ops():
-    import torch
+_calls = {}
 
-    if not hasattr(torch.ops.xinfer, "paged_attention_kv4"):
-        load_attention_ops(model="qwen3")
-    return torch.ops.xinfer
+
+def _call(name):
+    """The operator ``name``, loading the library on first use."""
+    found = _calls.get(name)
+    if found is None:
+        import torch
+
+        if not hasattr(torch.ops.xinfer, name):
+            load_attention_ops(model="qwen3")
+        found = _calls[name] = getattr(torch.ops.xinfer, name).default
+    return found
 
 
 def paged_kv4_cache(pages, kv_heads, page_size, dim, device):
@@ -63,7 +70,7 @@ def paged_kv_reserve(kv_before, kv_lengths, query_lengths, tokens, page_size, co
     whose pages were not to be had.  Slots of padded tokens are -1, their positions 0.  The call gives the same again
     for the same inputs.
     """
-    return _ops().paged_kv_reserve(kv_before, kv_lengths, query_lengths, tokens, page_size, counters, block_table,
+    return _call("paged_kv_reserve")(kv_before, kv_lengths, query_lengths, tokens, page_size, counters, block_table,
                                    free_pages)
 
 
@@ -72,12 +79,12 @@ def append_kv4(key, value, slots, cache):
 
     Slots outside the cache (-1 for padded tokens) are skipped.
     """
-    _ops().append_kv4(key, value, slots, *cache)
+    _call("append_kv4")(key, value, slots, *cache)
 
 
 def read_kv4(cache, slots):
     """What the cache holds at ``slots`` int64 [B,T]: (key, value) bf16 [B,Hkv,T,D], zero for slots outside it."""
-    return _ops().read_kv4(*cache, slots)
+    return _call("read_kv4")(*cache, slots)
 
 
 def qk_norm_rope_append_kv4(q, key, value, q_weight, k_weight, eps, weight_offset, cos, sin, slots, cache):
@@ -88,7 +95,7 @@ def qk_norm_rope_append_kv4(q, key, value, q_weight, k_weight, eps, weight_offse
     one), then the rotation of the first R features by ``cos``/``sin`` bf16 [B,T,R].  All in fp32; the query is rounded
     to bf16 once, the key goes to its 4 bits directly.
     """
-    return _ops().qk_norm_rope_append_kv4(q, key, value, q_weight, k_weight, float(eps), float(weight_offset), cos, sin,
+    return _call("qk_norm_rope_append_kv4")(q, key, value, q_weight, k_weight, eps, weight_offset, cos, sin,
                                           slots, *cache)
 
 
@@ -98,7 +105,7 @@ def paged_attention_kv4(q, cache, block_table, lengths, max_length, scale):
     ``lengths`` int32 [2,B] on the device, as ``paged_kv_reserve`` returns it.  ``max_length``: the host's bound on the
     rows' lengths (0: what the table can hold); it sizes the launch, and longer rows are read up to it.
     """
-    return _ops().paged_attention_kv4(q, *cache, block_table, lengths, int(max_length), float(scale))
+    return _call("paged_attention_kv4")(q, *cache, block_table, lengths, max_length, scale)
 
 
 def register_fakes():
