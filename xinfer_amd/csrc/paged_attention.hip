@@ -15,8 +15,8 @@ __global__ void __launch_bounds__(64 * kPagedWaves, D == 256 || NC == 2 ? 2 : 4)
 
 // Blocks below `few_items` take a decode item, the others a prefill item.
 template <int D>
-__global__ void __launch_bounds__(64 * paged_chunk_waves(D), 2) paged_both_kernel(const PagedArgs few, const PagedArgs many, int few_items) {
-  constexpr int WAVES = paged_chunk_waves(D), CHUNK = kPagedChunkLds<D>, DECODE = kPagedDecodeLds<D, WAVES>;
+__global__ void __launch_bounds__(64 * kPagedChunkWaves, 2) paged_both_kernel(const PagedArgs few, const PagedArgs many, int few_items) {
+  constexpr int WAVES = kPagedChunkWaves, CHUNK = kPagedChunkLds<D>, DECODE = kPagedDecodeLds<D, WAVES>;
   __shared__ __attribute__((aligned(1024))) char smem[CHUNK > DECODE ? CHUNK : DECODE];
   if ((int)blockIdx.x < few_items) {
     paged_decode_item<D, paged_decode_columns(D) / 16, WAVES>(few, blockIdx.x, smem);
@@ -29,7 +29,7 @@ __global__ void __launch_bounds__(64 * paged_chunk_waves(D), 2) paged_both_kerne
 
 // Prefill items alone.
 template <int D>
-__global__ void __launch_bounds__(64 * paged_chunk_waves(D), 2) paged_prefill_kernel(const PagedArgs a) {
+__global__ void __launch_bounds__(64 * kPagedChunkWaves, 2) paged_prefill_kernel(const PagedArgs a) {
   __shared__ __attribute__((aligned(1024))) char smem[kPagedChunkLds<D>];
   if constexpr (D == 256) paged_chunk_item_wide<D>(a, blockIdx.x, smem);
   else paged_chunk_item<D>(a, blockIdx.x, smem);
@@ -47,62 +47,71 @@ struct MergedRuns {
   }
 };
 
-// Joins the runs of rows that were cut, of either launch (blockIdx.z).  D/4 threads side by side take a query vector, 4
-// features each; a block has 256 / (D/4) such teams.  Decode rows have few vectors and many runs: a block takes one
-// vector, its teams every TEAMS-th run, and joins them in LDS.  Prefill rows have many vectors of few runs: a team takes a
-// vector of its own.  Either way four records are read at a time.
+// Joins the runs of rows that were cut, of either launch.  D/4 threads side by side take a query vector, 4 features
+// each; a block has 256 / (D/4) such teams.  Decode rows (blocks below few_blocks, the row counting slowest) have few
+// vectors and many runs: a block takes one vector, its teams every TEAMS-th run, and joins them in LDS.  Prefill rows
+// have many vectors of few runs: a team takes kMergeVectors of them, one after another.  Either way four records are
+// read at a time.
+constexpr int kMergeVectors = 4;
+
 template <int D>
-__global__ void __launch_bounds__(256) paged_merge_kernel(const PagedArgs few, const PagedArgs many) {
+__global__ void __launch_bounds__(256) paged_merge_kernel(const PagedArgs few, const PagedArgs many, int few_blocks,
+                                                          int few_per_row, int many_per_row) {
   constexpr int TEAMS = 256 / (D / 4);
   __shared__ f32x4 outs[TEAMS][D / 4];
   __shared__ f32x2 sums[TEAMS];
-  const PagedArgs &a = blockIdx.z == 0 ? few : many;
-  const bool together = a.tile <= 32;
-  const int per = together ? min(a.tile, a.T * a.G) : (a.tile + TEAMS - 1) / TEAMS;  // blocks of a (KV head, tile)
-  const int unit = blockIdx.x / per, first = blockIdx.x - unit * per;
+  const bool together = (int)blockIdx.x < few_blocks;
+  const PagedArgs &a = together ? few : many;
+  const uint32_t at = together ? blockIdx.x : blockIdx.x - few_blocks, per_row = together ? few_per_row : many_per_row;
+  const uint32_t row = at / per_row, in_row = at - row * per_row;
+  const uint32_t per = together ? min(a.tile, a.T * a.G) : (a.tile + TEAMS * kMergeVectors - 1) / (TEAMS * kMergeVectors);
+  const uint32_t unit = in_row / per, first = in_row - unit * per;
   const int tile = unit / a.cache.Hkv, h = unit - tile * a.cache.Hkv;
   PagedItem it;
-  paged_row_items(a, blockIdx.y, it);
+  paged_row_items(a, row, it);
+  if (it.nsplit <= 1 || tile >= it.tiles) return;
   const int team = threadIdx.x / (D / 4), f = threadIdx.x % (D / 4);
-  const int column = together ? first : first * TEAMS + team;
-  if (it.nsplit <= 1 || tile >= it.tiles || (together ? first : first * TEAMS) >= min(it.count * a.G - tile * a.tile, a.tile)) return;
-  const bool there = column < min(it.count * a.G - tile * a.tile, a.tile);
-  const int64_t record0 = ((int64_t)it.begin + (int64_t)tile * it.nsplit * a.cache.Hkv + h) * a.tile + (there ? column : 0);
+  const int vectors = min(it.count * a.G - tile * a.tile, a.tile);
+  if (together && (int)first >= vectors) return;
   const int64_t step = (int64_t)a.cache.Hkv * a.tile;
-  MergedRuns r{kLowest, 0.0f, f32x4{0.0f, 0.0f, 0.0f, 0.0f}};
+  const int64_t record0 = ((int64_t)it.begin + (int64_t)tile * it.nsplit * a.cache.Hkv + h) * a.tile;
   const int begin = together ? team : 0, stride = together ? TEAMS : 1;
-  for (int s0 = begin; s0 < it.nsplit; s0 += 4 * stride) {
-    f32x2 ml[4];
-    f32x4 part[4];
+  for (int n = 0; n < (together ? 1 : kMergeVectors); ++n) {
+    const int column = together ? first : (first * kMergeVectors + n) * TEAMS + team;
+    if (column >= vectors) return;
+    MergedRuns r{kLowest, 0.0f, f32x4{0.0f, 0.0f, 0.0f, 0.0f}};
+    for (int s0 = begin; s0 < it.nsplit; s0 += 4 * stride) {
+      f32x2 ml[4];
+      f32x4 part[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int64_t record = record0 + min(s0 + e * stride, it.nsplit - 1) * step;
-      ml[e] = *as_global(reinterpret_cast<const f32x2 *>(a.part_ml + 2 * record));
-      part[e] = *as_global(reinterpret_cast<const f32x4 *>(a.part_o + record * D + 4 * f));
+      for (int e = 0; e < 4; ++e) {
+        const int64_t record = record0 + column + min(s0 + e * stride, it.nsplit - 1) * step;
+        ml[e] = *as_global(reinterpret_cast<const f32x2 *>(a.part_ml + 2 * record));
+        part[e] = *as_global(reinterpret_cast<const f32x4 *>(a.part_o + record * D + 4 * f));
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (s0 + e * stride < it.nsplit) r.add(ml[e].x, ml[e].y, part[e]);
     }
+    if (together) {
+      outs[team][f] = r.out;
+      if (f == 0) sums[team] = f32x2{r.best, r.total};
+      __syncthreads();
+      if (team != 0) return;
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (s0 + e * stride < it.nsplit) r.add(ml[e].x, ml[e].y, part[e]);
+      for (int e = 1; e < TEAMS; ++e) r.add(sums[e].x, sums[e].y, outs[e][f]);
+    }
+    const int j = tile * a.tile + column, t = j / a.G;
+    r.out *= r.total == 0.0f ? 0.0f : 1.0f / r.total;
+    *as_global(reinterpret_cast<u32x2 *>(
+        a.out + (((int64_t)row * a.T + t) * a.Hq + h * a.G + (j - t * a.G)) * D + 4 * f)) =
+        u32x2{pack_bf16x2(r.out[0], r.out[1]), pack_bf16x2(r.out[2], r.out[3])};
   }
-  if (together) {
-    outs[team][f] = r.out;
-    if (f == 0) sums[team] = f32x2{r.best, r.total};
-    __syncthreads();
-    if (team != 0) return;
-#pragma unroll
-    for (int e = 1; e < TEAMS; ++e) r.add(sums[e].x, sums[e].y, outs[e][f]);
-  }
-  if (!there) return;
-  const int j = tile * a.tile + column, t = j / a.G;
-  r.out *= r.total == 0.0f ? 0.0f : 1.0f / r.total;
-  *as_global(reinterpret_cast<u32x2 *>(
-      a.out + (((int64_t)it.row * a.T + t) * a.Hq + h * a.G + (j - t * a.G)) * D + 4 * f)) =
-      u32x2{pack_bf16x2(r.out[0], r.out[1]), pack_bf16x2(r.out[2], r.out[3])};
 }
 
 template <int D>
 static hipError_t launch_d(const PagedLaunches &l, hipStream_t stream) {
-  const dim3 block(64 * paged_chunk_waves(D)), few_block(64 * kPagedWaves);
+  const dim3 block(64 * kPagedChunkWaves), few_block(64 * kPagedWaves);
   const PagedArgs &few = l.few.a, &many = l.many.a;
   if (l.few.items > 0 && l.many.items > 0) {
     hipLaunchKernelGGL((paged_both_kernel<D>), dim3(l.few.items + l.many.items), block, 0, stream, few, many, (int)l.few.items);
@@ -115,14 +124,12 @@ static hipError_t launch_d(const PagedLaunches &l, hipStream_t stream) {
     hipLaunchKernelGGL((paged_decode_kernel<D, 1>), dim3(l.few.items), few_block, 0, stream, few);
   }
   if (l.bytes() > 0) {
-    constexpr int TEAMS = 256 / (D / 4);
-    const unsigned heads = few.cache.Hkv;
-    const unsigned few_blocks = l.few.bytes > 0 ? heads * l.few.tiles * std::min(few.tile, few.T * few.G) : 0;
-    const unsigned many_blocks = l.many.bytes > 0 ? heads * l.many.tiles * ((many.tile + TEAMS - 1) / TEAMS) : 0;
-    const unsigned blocks = std::max(few_blocks, many_blocks);
-    const bool both = l.few.bytes > 0 && l.many.bytes > 0;
-    const PagedArgs &one = l.few.bytes > 0 ? few : many;
-    hipLaunchKernelGGL((paged_merge_kernel<D>), dim3(blocks, few.B, both ? 2 : 1), dim3(256), 0, stream, one, many);
+    constexpr int VECTORS = 256 / (D / 4) * kMergeVectors;
+    const int heads = few.cache.Hkv, rows = few.B;
+    const int few_per_row = l.few.bytes > 0 ? heads * l.few.tiles * std::min(few.tile, few.T * few.G) : 0;
+    const int many_per_row = l.many.bytes > 0 ? heads * l.many.tiles * ((many.tile + VECTORS - 1) / VECTORS) : 0;
+    hipLaunchKernelGGL((paged_merge_kernel<D>), dim3((unsigned)rows * (few_per_row + many_per_row)), dim3(256), 0, stream, few,
+                       many, rows * few_per_row, few_per_row, many_per_row);
   }
   return hipGetLastError();
 }

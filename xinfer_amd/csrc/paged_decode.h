@@ -119,6 +119,25 @@ struct GroupLoads {
   }
 };
 
+// The largest of three; a NaN counts for nothing.
+__device__ __forceinline__ float max3(float x, float y, float z) { return fmaxf(fmaxf(x, y), z); }
+
+// STEPS products whose A operands come from LDS, DEPTH reads ahead of their use.  The order is kept: left alone, the
+// compiler reads one operand at a time and every product waits for LDS.
+template <int STEPS, int DEPTH, typename Get, typename Use>
+__device__ __forceinline__ void pipelined(Get get, Use use) {
+  bf16x8 x[DEPTH];
+#pragma unroll
+  for (int k = 0; k < DEPTH && k < STEPS; ++k) x[k] = get(k);
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int k = 0; k < STEPS; ++k) {
+    use(k, x[k % DEPTH]);
+    if (k + DEPTH < STEPS) x[k % DEPTH] = get(k + DEPTH);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
 // A query column's operands: the two e4m3 terms of each chunk, their scale bytes (terms' in bytes 0 and 1).
 template <int D>
 struct QueryOperand {
@@ -304,14 +323,21 @@ __device__ __forceinline__ void paged_decode_item(const PagedArgs &a, int index,
       if (u == 1) in.values(a, load_page, it.h, place(next));
       asm volatile("" ::: "memory");
       __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int d = 0; d < S::DT; ++d) {
-        if (d % 4 == 0) __builtin_amdgcn_sched_barrier(0);
-        const bf16x8 v = in.get(d);
+      auto use = [&](int d, const bf16x8 &v) {
 #pragma unroll
         for (int n = 0; n < NC; ++n)
           o[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
               v, as_bf16x8(u32x4{pw[n][u][0], pw[n][u][1], pw[n][u][2], pw[n][u][3]}), o[n][d], 0, 0, 0);
+      };
+      if constexpr (D == 256 || NC == 2) {
+        pipelined<S::DT, 4>([&](int d) { return in.get(d); }, use);
+      } else {
+        // Four waves a SIMD fill each other's waits, and there are no registers to read ahead.
+#pragma unroll
+        for (int d = 0; d < S::DT; ++d) {
+          if (d % 4 == 0) __builtin_amdgcn_sched_barrier(0);
+          use(d, in.get(d));
+        }
       }
       asm volatile("" ::: "memory");
       __builtin_amdgcn_sched_barrier(0);

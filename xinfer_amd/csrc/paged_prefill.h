@@ -1,14 +1,14 @@
 // Attention over the paged 4-bit cache for rows of many query vectors a KV head: prompt chunks.
 //
 // A block takes an item (paged_plan.h): 128 query vectors of a (row, KV head) over a run of keys in 64-key groups.  Up
-// to 128 features it has 4 waves of 32 vectors each (paged_chunk_item).  A wave reads the group's keys as they lie in the cache, as the A operand of the scaled
+// to 128 features each half of its 8 waves takes all of them, 32 a wave, over every other group (paged_chunk_item).  A wave reads the group's keys as they lie in the cache, as the A operand of the scaled
 // 32x32x64 product against its queries' two e4m3 terms (paged_mfma.h): row m of tile t (of two) is key 2 m + t, so a
 // lane's two keys have their scales in neighbouring bytes.  A lane (column q, half h) then holds 32 scores of its query,
 // and for each 16 keys 8 neighbouring ones, which is the B operand of the bf16 PV product: nothing of the softmax
 // crosses lanes but the maximum and, at the end, the sum of the two halves.
 //
-// The block turns the group's values into bf16 (exact) in LDS together, one group ahead, and every wave reads
-// them transposed as the A operand.  One barrier a group.
+// The waves of a group turn its values into bf16 (exact) in LDS together, a group ahead, and each reads them transposed
+// as the A operand.  One barrier a round.
 //
 // 256 features of 32 vectors would take 128 registers for the output and 64 for the queries, which leaves no two
 // waves a SIMD.  There 8 waves take 16 vectors each (paged_chunk_item_wide), with the products and layouts of the
@@ -21,10 +21,8 @@
 
 namespace xattn {
 
-constexpr int kChunkWaves = 4, kChunkThreads = 64 * kChunkWaves;
-constexpr int kWideWaves = 8;
-// Waves of a prefill block.
-constexpr int paged_chunk_waves(int dim) { return dim == 256 ? kWideWaves : kChunkWaves; }
+constexpr int kPagedChunkWaves = 8;  // of a prefill block
+constexpr int kChunkWaves = kPagedChunkWaves / 2, kChunkThreads = 64 * kChunkWaves;  // of half a block
 
 template <int D>
 struct ChunkShape {
@@ -32,7 +30,6 @@ struct ChunkShape {
   static constexpr int DT = D / 32;                                  // 32-feature tiles of the output
   static constexpr int ROW = 2 * D, STAGE = 64 * ROW;                // staged values of a group
   static constexpr int UNITS = 64 * (D / 32);                        // (key, block) units of a group
-  static constexpr int VL = (UNITS + kChunkThreads - 1) / kChunkThreads;
 };
 
 // XOR of the 16-byte chunk index of staged row r: the four rows that a half's transposing read takes lie in different
@@ -42,20 +39,31 @@ __device__ __forceinline__ int chunk_swizzle(int r) {
   return D == 64 ? 5 * ((r >> 1) & 1) : 5 * (r & 3);
 }
 
-// LDS of a prefill block: staged groups.
+template <bool B>
+struct Flag {
+  static constexpr bool value = B;
+};
+
+// The block's barrier for what its waves have stored in LDS.  Loads from memory stay under way (__syncthreads would wait
+// for them, and with that for a memory round trip every group).
+__device__ __forceinline__ void staged_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory"); }
+
+// LDS of a prefill block: staged groups, two for each half of the waves, and the second half's maxima and sums (256
+// features: three groups for all waves).
 template <int D>
-constexpr int kPagedChunkLds = (D == 256 ? 3 : 2) * 64 * 2 * D;
+constexpr int kPagedChunkLds = D == 256 ? 3 * 64 * 2 * D : 4 * 64 * 2 * D + 64 * kChunkWaves * 8;
 
 // Item `index` of the plan, by the whole block; smem: kPagedChunkLds bytes, 1024-byte aligned.
 template <int D>
 __device__ __forceinline__ void paged_chunk_item(const PagedArgs &a, int index, char *smem) {
   using S = ChunkShape<D>;
   constexpr int COLS = 32 * kChunkWaves;
-  const int tid = threadIdx.x, lane = tid & 63, m = lane & 31, h = lane >> 5;
+  const int tid = threadIdx.x & (kChunkThreads - 1), lane = tid & 63, m = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int side = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kChunkThreads);  // which groups: every other one
   PagedItem it;
   if (!paged_item(a, index, it)) return;
-  paged_zero_padded<D, kChunkThreads>(a, it);
+  paged_zero_padded<D, 2 * kChunkThreads>(a, it);
 
   // This wave's queries.
   const int vectors = it.count * a.G, j = it.tile * COLS + 32 * wave + m;
@@ -69,26 +77,32 @@ __device__ __forceinline__ void paged_chunk_item(const PagedArgs &a, int index, 
   const int tile_end = it.length - it.count + (min(it.tile * COLS + COLS, vectors) - 1) / a.G + 1;
   const int group_end = min(it.group_end, (tile_end + kGroupKeys - 1) / kGroupKeys);
 
-  u32x4 first[S::KS][2], second[S::KS][2];
+  u32x4 first[S::KS][2], second[S::KS][2], qx[S::KS][2][2];
   int qscale[S::KS];
   {
     const uint16_t *const q = a.q.p + it.row * a.q.sb + head * a.q.sh + t * a.q.st;
+#pragma unroll
+    for (int s = 0; s < S::KS; ++s)
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) qx[s][p][e] = there ? load16(q + 64 * s + 32 * p + 16 * h + 8 * e) : u32x4{0, 0, 0, 0};
+  }
+  auto convert_queries = [&]() {
 #pragma unroll
     for (int s = 0; s < S::KS; ++s) {
       int b[2];
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
-        const uint16_t *const at = q + 64 * s + 32 * p + 16 * h;
-        const u32x4 x0 = there ? load16(at) : u32x4{0, 0, 0, 0}, x1 = there ? load16(at + 8) : u32x4{0, 0, 0, 0};
-        const uint32_t top = largest(x1, largest(x0, 0u));
+        const uint32_t top = largest(qx[s][p][1], largest(qx[s][p][0], 0u));
         const auto r = __builtin_amdgcn_permlane32_swap(top, top, false, false);  // the block's other half
         b[p] = query_scale(max(r[0], r[1]));
-        split_query(x0, x1, b[p], first[s][p], second[s][p]);
+        split_query(qx[s][p][0], qx[s][p][1], b[p], first[s][p], second[s][p]);
       }
       const int mine = h == 0 ? b[0] : b[1];
       qscale[s] = mine | (mine == 255 ? 255 : mine - 4) << 8;
     }
-  }
+  };
 
   f32x16 o[S::DT];
 #pragma unroll
@@ -122,116 +136,171 @@ __device__ __forceinline__ void paged_chunk_item(const PagedArgs &a, int index, 
 #pragma unroll
     for (int s = 0; s < S::KS; ++s) ks[s] = *as_global(reinterpret_cast<const uint16_t *>(scales + 2 * s * size + key_scale_at));
   };
-  // Values of a group: unit w of a thread is (key, block) = tid + w * threads, the block counting fastest.
-  u32x4 v[S::VL];
-  uint32_t vs[S::VL];
-  const int block = tid % (D / 32), row0 = tid / (D / 32);
-  constexpr int ROWS = kChunkThreads / (D / 32);  // rows a load covers
-  const uint32_t value_at = row0 * (D / 2) + 16 * block, value_scale_at = block * size + row0;
-  const uint32_t stage0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)smem;
-  const bool stages = S::UNITS >= kChunkThreads || tid < S::UNITS;
-  const uint32_t put_at = stage0 + row0 * S::ROW + ((4 * block) ^ chunk_swizzle<D>(row0) ^ (block >> 2)) * 16;
+  // Values of a group: a thread of the half stages one (key, block), the block counting fastest.
+  static_assert(S::UNITS <= kChunkThreads, "one unit a thread");
+  u32x4 v;
+  uint32_t vs;
+  const int block = tid % (D / 32), row = tid / (D / 32);
+  const uint32_t value_at = 16 * tid, value_scale_at = block * size + row;
+  const uint32_t stage = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)smem + side * 2 * S::STAGE;
+  const bool stages = S::UNITS == kChunkThreads || tid < S::UNITS;
+  const uint32_t put_at = stage + row * S::ROW + ((4 * block) ^ chunk_swizzle<D>(row)) * 16;
   auto load_values = [&](int group, int page) {
     const int64_t hd = (int64_t)max(page, 0) * a.cache.Hkv + it.h;
     const uint8_t *const codes = a.cache.value + (hd * size + place(group)) * (D / 2);
     const uint8_t *const scales = a.cache.value_scale + hd * (D / 32) * size + place(group);
     if (stages) {
-#pragma unroll
-      for (int w = 0; w < S::VL; ++w) {
-        v[w] = *as_global(reinterpret_cast<const u32x4 *>(codes + w * ROWS * (D / 2) + value_at));
-        vs[w] = *as_global(scales + w * ROWS + value_scale_at);
-      }
+      v = *as_global(reinterpret_cast<const u32x4 *>(codes + value_at));
+      vs = *as_global(scales + value_scale_at);
     }
   };
   auto put_values = [&](int buffer) {
     if (stages) {
+      const float scale = kv4_scale_value(min((int)vs, kKv4MaxScale));
 #pragma unroll
-      for (int w = 0; w < S::VL; ++w) {
-        const float scale = kv4_scale_value(min((int)vs[w], kKv4MaxScale));
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-          *(__attribute__((address_space(3))) u32x4 *)((put_at ^ (16 * c)) + w * ROWS * S::ROW + buffer * S::STAGE) =
-              kv4_values(v[w][c], scale);
-      }
+      for (int c = 0; c < 4; ++c)
+        *(__attribute__((address_space(3))) u32x4 *)((put_at ^ (16 * c)) + buffer * S::STAGE) = kv4_values(v[c], scale);
     }
   };
   // Transposing reads: lane (m, h) gets feature 32 d + m of keys 16 b + 8 h + 0..7.
   const int x = 8 * h + ((lane & 15) >> 2);
-  const uint32_t get_at = stage0 + x * S::ROW + ((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ chunk_swizzle<D>(x)) * 16 + 8 * (lane & 1);
+  uint32_t get_at = stage + x * S::ROW + ((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ chunk_swizzle<D>(x)) * 16 + 8 * (lane & 1);
 
-  int group = it.group_begin;
-  if (group < group_end) {
-    int page = page_of(group), next_page = page_of(group + 1);
-    load_values(group, page);
-    load_keys(group, page);
-    put_values(0);
-    load_values(group + 1, next_page);
-    for (int buffer = 0; group < group_end; ++group, buffer ^= 1) {
-      asm volatile("" : "+v"(key_at), "+v"(key_scale_at));
-      const int after_page = page_of(group + 2);
-      // Every wave has stored its part of this group's values, and is done with the group before.
-      __syncthreads();
-      put_values(buffer ^ 1);
-      load_values(group + 2, after_page);
-      const bool active = group * kGroupKeys < none_see && page >= 0;  // uniform in the wave
-      f32x16 s[2];
+  f32x16 s[2];
+  uint32_t pw[4][4];
+  // A group's scores, then the loads of the half's next keys.
+  auto scores = [&](int next, int next_page) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[0][r] = s[1][r] = 0.0f;
+    for (int r = 0; r < 16; ++r) s[0][r] = s[1][r] = 0.0f;
 #pragma unroll
-      for (int i = 0; i < S::KS; ++i) {
-        s[0] = mfma32_fp4<0, 0>(k[0][i], first[i], s[0], (int)ks[i], qscale[i]);
-        s[0] = mfma32_fp4<0, 1>(k[0][i], second[i], s[0], (int)ks[i], qscale[i]);
-        s[1] = mfma32_fp4<1, 0>(k[1][i], first[i], s[1], (int)ks[i], qscale[i]);
-        s[1] = mfma32_fp4<1, 1>(k[1][i], second[i], s[1], (int)ks[i], qscale[i]);
-      }
-      asm volatile("" : "+v"(s[0]), "+v"(s[1]) : : "memory");
-      load_keys(group + 1, next_page);
-      page = next_page, next_page = after_page;
-      if (!active) continue;
-      // s[x][r] is key 16 (r / 4) + 8 h + 2 (r % 4) + x of the group.
-      if (group * kGroupKeys + kGroupKeys - 1 > all_see) {
-        const int key = group * kGroupKeys + 8 * h;
+    for (int i = 0; i < S::KS; ++i) {
+      s[0] = mfma32_fp4<0, 0>(k[0][i], first[i], s[0], (int)ks[i], qscale[i]);
+      s[1] = mfma32_fp4<1, 0>(k[1][i], first[i], s[1], (int)ks[i], qscale[i]);
+      s[0] = mfma32_fp4<0, 1>(k[0][i], second[i], s[0], (int)ks[i], qscale[i]);
+      s[1] = mfma32_fp4<1, 1>(k[1][i], second[i], s[1], (int)ks[i], qscale[i]);
+    }
+    asm volatile("" : "+v"(s[0]), "+v"(s[1]) : : "memory");
+    load_keys(next, next_page);
+  };
+  // Weights of a group: s[x][r] is key 16 (r / 4) + 8 h + 2 (r % 4) + x.
+  auto weights = [&](int group, int page) {
+    if (group * kGroupKeys + kGroupKeys - 1 > all_see || page < 0) {
+      const int key = group * kGroupKeys + 8 * h, last = page < 0 ? -1 : last_key;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int at = key + 16 * (r / 4) + 2 * (r % 4);
-          s[0][r] = at <= last_key ? s[0][r] : -INFINITY;
-          s[1][r] = at + 1 <= last_key ? s[1][r] : -INFINITY;
-        }
-      }
-      float best = fmaxf(s[0][0], s[1][0]);
-#pragma unroll
-      for (int r = 1; r < 16; ++r) best = fmaxf(best, fmaxf(s[0][r], s[1][r]));
-      best = fmaxf(top, pair_max32(best) * a.scale_log2);
-      if (__any(best > top)) {
-        const float keep = fast_exp2(top - best);
-        sum *= keep;
-#pragma unroll
-        for (int d = 0; d < S::DT; ++d) o[d] *= keep;
-        top = best;
-      }
-      const uint32_t get = get_at + buffer * S::STAGE;
-#pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        uint32_t pw[4];
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const float p0 = fast_exp2(fmaf(s[0][4 * b + w], a.scale_log2, -top)), p1 = fast_exp2(fmaf(s[1][4 * b + w], a.scale_log2, -top));
-          sum += p0 + p1;
-          pw[w] = pack_bf16x2(p0, p1);
-        }
-        const bf16x8 weights = as_bf16x8(u32x4{pw[0], pw[1], pw[2], pw[3]});
-#pragma unroll
-        for (int d = 0; d < S::DT; ++d) {
-          const uint32_t at = (get ^ (64 * d) ^ (d >= 4 ? 16 : 0)) + 16 * b * S::ROW;
-          const u32x2 lo = read_transposed(at), hi = read_transposed(at + 4 * S::ROW);
-          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(u32x4{lo.x, lo.y, hi.x, hi.y}), weights, o[d], 0, 0, 0);
-        }
+      for (int r = 0; r < 16; ++r) {
+        const int at = key + 16 * (r / 4) + 2 * (r % 4);
+        s[0][r] = at <= last ? s[0][r] : -INFINITY;
+        s[1][r] = at + 1 <= last ? s[1][r] : -INFINITY;
       }
     }
+    float best = max3(s[0][0], s[1][0], s[0][1]);
+#pragma unroll
+    for (int r = 1; r < 16; ++r) best = max3(best, s[1][r], s[0][(r + 1) & 15]);
+    best = fmaxf(top, pair_max32(best) * a.scale_log2);
+    if (__any(best > top)) {
+      const float keep = fast_exp2(top - best);
+      sum *= keep;
+#pragma unroll
+      for (int d = 0; d < S::DT; ++d) o[d] *= keep;
+      top = best;
+    }
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float p0 = fast_exp2(fmaf(s[0][4 * b + w], a.scale_log2, -top)), p1 = fast_exp2(fmaf(s[1][4 * b + w], a.scale_log2, -top));
+        sum += p0 + p1;
+        pw[b][w] = pack_bf16x2(p0, p1);
+      }
+  };
+  auto output = [&](int buffer) {
+    const uint32_t get = get_at + buffer * S::STAGE;
+    pipelined<4 * S::DT, 4>(
+        [&](int n) {
+          const int b = n / S::DT, d = n % S::DT;
+          const uint32_t at = (get ^ (64 * d)) + 16 * b * S::ROW;
+          const u32x2 lo = read_transposed(at), hi = read_transposed(at + 4 * S::ROW);
+          return as_bf16x8(u32x4{lo.x, lo.y, hi.x, hi.y});
+        },
+        [&](int n, const bf16x8 &w) {
+          const int b = n / S::DT, d = n % S::DT;
+          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w, as_bf16x8(u32x4{pw[b][0], pw[b][1], pw[b][2], pw[b][3]}), o[d], 0, 0, 0);
+        });
+  };
+  // The two halves of the waves take alternate groups.  Waves w and w + 4 share a SIMD, and between two barriers the
+  // first half computes weights, then the matrix products (this group's output, its next one's scores), the second
+  // half the products first (its last group's output, this one's scores), then weights: one's matrix work runs
+  // beside the other's vector work.  Each half has a loop of its own: in a common one the compiler's waits for
+  // loads would be those of either order.
+  const int begin = it.group_begin, rounds = (group_end - begin + 1) / 2;
+  auto sweep = [&](auto order) {
+    constexpr bool AHEAD = decltype(order)::value;
+    const int start = begin + (AHEAD ? 0 : 1);
+    int page = page_of(start), next_page = page_of(start + 2);
+    load_values(start, page);
+    load_keys(start, page);
+    convert_queries();
+    if constexpr (AHEAD) {
+      put_values(0);
+      load_values(start + 2, next_page);
+      scores(start + 2, next_page);
+    }
+    int group = start;
+    for (int round = 0; round < rounds; ++round, group += 2) {
+      asm volatile("" : "+v"(key_at), "+v"(key_scale_at), "+v"(get_at));
+      const int after_page = page_of(group + 4);
+      const bool active = group * kGroupKeys < none_see && group < group_end;  // uniform in the wave
+      staged_barrier();  // the values that this round's outputs read are in LDS
+      if constexpr (AHEAD) {
+        put_values((round & 1) ^ 1);
+        load_values(group + 4, after_page);
+        if (active) {
+          weights(group, page);
+          output(round & 1);
+        }
+        scores(group + 4, after_page);
+      } else {
+        if (round > 0 && (group - 2) * kGroupKeys < none_see) output((round & 1) ^ 1);
+        scores(group + 2, next_page);
+        put_values(round & 1);
+        load_values(group + 2, next_page);
+        if (active) weights(group, page);
+      }
+      page = next_page, next_page = after_page;
+    }
+    if constexpr (!AHEAD) {
+      staged_barrier();
+      if (group - 2 < group_end && (group - 2) * kGroupKeys < none_see) output((rounds & 1) ^ 1);
+    } else {
+      staged_barrier();
+    }
+  };
+  if (rounds > 0) {
+    if (side == 0) sweep(Flag<true>{});
+    else sweep(Flag<false>{});
   }
 
+  // The second half hands its output over in LDS, a word of all lanes side by side.
   sum = pair_sum32(sum);
-  if (!there) return;
+  float *const over = reinterpret_cast<float *>(smem) + wave * (32 * D) + lane;
+  f32x2 *const over_ml = reinterpret_cast<f32x2 *>(smem + 4 * S::STAGE) + 64 * wave + lane;
+  __syncthreads();
+  if (side == 1) {
+    *over_ml = f32x2{top, sum};
+#pragma unroll
+    for (int d = 0; d < S::DT; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) over[(16 * d + r) * 64] = o[d][r];
+  }
+  __syncthreads();
+  if (side == 1 || !there) return;
+  const f32x2 other = *over_ml;
+  const float best = fmaxf(top, other.x), mine = fast_exp2(top - best), theirs = fast_exp2(other.x - best);
+  sum = sum * mine + other.y * theirs;
+#pragma unroll
+  for (int d = 0; d < S::DT; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[d][r] = o[d][r] * mine + over[(16 * d + r) * 64] * theirs;
   // o[d][r] is feature 32 d + 8 (r / 4) + 4 h + r % 4.
   if (it.nsplit > 1) {
     const int64_t record = (int64_t)index * COLS + 32 * wave + m;
@@ -241,7 +310,7 @@ __device__ __forceinline__ void paged_chunk_item(const PagedArgs &a, int index, 
       for (int r = 0; r < 4; ++r)
         *as_global(reinterpret_cast<f32x4 *>(a.part_o + record * D + 32 * d + 8 * r + 4 * h)) =
             f32x4{o[d][4 * r], o[d][4 * r + 1], o[d][4 * r + 2], o[d][4 * r + 3]};
-    if (h == 0) *as_global(reinterpret_cast<f32x2 *>(a.part_ml + 2 * record)) = f32x2{top, sum};
+    if (h == 0) *as_global(reinterpret_cast<f32x2 *>(a.part_ml + 2 * record)) = f32x2{best, sum};
   } else {
     const float by = sum == 0.0f ? 0.0f : 1.0f / sum;
     uint16_t *const out = a.out + (((int64_t)it.row * a.T + t) * a.Hq + head) * D + 4 * h;
@@ -258,7 +327,7 @@ __device__ __forceinline__ void paged_chunk_item(const PagedArgs &a, int index, 
 template <int D>
 __device__ __forceinline__ void paged_chunk_item_wide(const PagedArgs &a, int index, char *smem) {
   using S = PagedShape<D>;
-  constexpr int WAVES = kWideWaves, THREADS = 64 * WAVES, COLS = 16 * WAVES, BLOCKS = D / 32, STAGE = 64 * S::ROW;
+  constexpr int WAVES = kPagedChunkWaves, THREADS = 64 * WAVES, COLS = 16 * WAVES, BLOCKS = D / 32, STAGE = 64 * S::ROW;
   static_assert(64 * BLOCKS == THREADS, "a thread stages one block of one key");
   const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -334,9 +403,10 @@ __device__ __forceinline__ void paged_chunk_item_wide(const PagedArgs &a, int in
 #pragma unroll
         for (int i = 0; i < 4; ++i) s[u][i] = at + 4 * i + u <= last ? s[u][i] : -INFINITY;
     }
-    float best = fmaxf(fmaxf(s[0][0], s[1][0]), fmaxf(s[2][0], s[3][0]));
+    float best = max3(s[0][0], s[1][0], s[2][0]);
+    best = max3(best, s[3][0], s[0][1]);
 #pragma unroll
-    for (int i = 1; i < 4; ++i) best = fmaxf(best, fmaxf(fmaxf(s[0][i], s[1][i]), fmaxf(s[2][i], s[3][i])));
+    for (int i = 1; i < 4; ++i) best = max3(max3(best, s[1][i], s[2][i]), s[3][i], s[0][(i + 1) & 3]);
     best = fmaxf(top, pair_max32(pair_max16(best)) * a.scale_log2);
     if (__any(best > top)) {
       const float keep = fast_exp2(top - best);
@@ -357,45 +427,47 @@ __device__ __forceinline__ void paged_chunk_item_wide(const PagedArgs &a, int in
   };
   auto output = [&](int buffer) {
     const uint32_t get = get_at + buffer * STAGE;
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const bf16x8 w = as_bf16x8(u32x4{pw[u][0], pw[u][1], pw[u][2], pw[u][3]});
-#pragma unroll
-      for (int d = 0; d < S::DT; ++d) {
-        const uint32_t at = (get ^ (32 * d) ^ (d >= 8 ? 16 : 0)) + 8 * u * S::ROW;
-        const u32x2 lo = read_transposed(at), hi = read_transposed(at + 4 * S::ROW);
-        o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(u32x4{lo.x, lo.y, hi.x, hi.y}), w, o[d], 0, 0, 0);
-      }
-    }
+    pipelined<2 * S::DT, 4>(
+        [&](int k) {
+          const int u = k / S::DT, d = k % S::DT;
+          const uint32_t at = (get ^ (32 * d) ^ (d >= 8 ? 16 : 0)) + 8 * u * S::ROW;
+          const u32x2 lo = read_transposed(at), hi = read_transposed(at + 4 * S::ROW);
+          return as_bf16x8(u32x4{lo.x, lo.y, hi.x, hi.y});
+        },
+        [&](int k, const bf16x8 &x) {
+          const int u = k / S::DT, d = k % S::DT;
+          o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, as_bf16x8(u32x4{pw[u][0], pw[u][1], pw[u][2], pw[u][3]}), o[d], 0, 0, 0);
+        });
   };
   // Waves w and w + 4 share a SIMD.  Between two barriers the first half of the waves computes weights, then the
   // matrix products (this group's output, the next one's scores); the second half the products first (the last
   // group's output, this one's scores), then weights: one's matrix work runs beside the other's vector work.  So three
   // groups' values are staged: the last, this and the next one.
-  const bool ahead = wave < WAVES / 2;
+  // Each half has a loop of its own: in a common one the compiler's waits for loads would be those of either order.
   const int begin = it.group_begin;
-  if (begin < group_end) {
+  auto sweep = [&](auto order) {
+    constexpr bool AHEAD = decltype(order)::value;
     int page = page_of(begin), next_page = page_of(begin + 1);
     load_values(begin, page);
     in.keys(a, max(page, 0), it.h, place(begin));
     q.convert(qx, m, g);
     put_values(0);
     load_values(begin + 1, next_page);
-    if (ahead) scores(begin + 1, next_page);
+    if constexpr (AHEAD) scores(begin + 1, next_page);
     int last = 2, now = 0, next = 1;  // staged groups' buffers
     for (int group = begin; group < group_end; ++group) {
       asm volatile("" : "+v"(in.key_at), "+v"(in.key_scale_at), "+v"(get_at));
       const int after_page = page_of(group + 2);
       const bool active = group * kGroupKeys < none_see;  // uniform in the wave
-      __syncthreads();  // every wave has stored its part of this group's values
-      if (!ahead) {
+      staged_barrier();  // every wave has stored its part of this group's values
+      if constexpr (!AHEAD) {
         if (group > begin && (group - 1) * kGroupKeys < none_see) output(last);
         scores(group + 1, next_page);
       }
       put_values(next);
       load_values(group + 2, after_page);
       if (active) weights(group, page);
-      if (ahead) {
+      if constexpr (AHEAD) {
         if (active) output(now);
         scores(group + 2, after_page);
       }
@@ -403,7 +475,13 @@ __device__ __forceinline__ void paged_chunk_item_wide(const PagedArgs &a, int in
       const int free = last;
       last = now, now = next, next = free;
     }
-    if (!ahead && (group_end - 1) * kGroupKeys < none_see) output(last);
+    if constexpr (!AHEAD) {
+      if ((group_end - 1) * kGroupKeys < none_see) output(last);
+    }
+  };
+  if (begin < group_end) {
+    if (wave < WAVES / 2) sweep(Flag<true>{});
+    else sweep(Flag<false>{});
   }
 
   sum = pair_sum32(pair_sum16(sum));
