@@ -46,45 +46,80 @@ __global__ void __launch_bounds__(256) read_kv4_kernel(const Kv4ReadArgs a) {
 }
 
 // y = x * rsqrt(mean(x^2) + eps) * (weight + offset); of its first R features, the first half turns to
-// y_i cos_i - y_{i + R/2} sin_i and the second to y_i cos_i + y_{i - R/2} sin_i.  A query is rounded once, from fp32 to
-// bf16.  A key goes to its codes, where a value next to a border changes by a whole step of the grid: it is computed in
-// 64 bits, so that the codes are those of the definition.  The rotation's other half is read from memory again (a line
-// this wave reads anyway) and normalised here, which takes no exchange between lanes.
-__device__ __forceinline__ double wide_shuffle(double x, int mask) {
-  return __hiloint2double(__shfl_xor(__double2hiint(x), mask), __shfl_xor(__double2loint(x), mask));
-}
-template <int LPR, typename F>
-__device__ __forceinline__ void norm_rope_row(const uint16_t *x, const uint16_t *weight, const uint16_t *cos,
-                                              const uint16_t *sin, float eps, float offset, int R, int c,
-                                              float (&y)[8]) {
-  const int half = R / 16;  // chunks of half the rotated features
-  const bool turned = c < 2 * half;
-  const int other = c < half ? c + half : (turned ? c - half : c);
-  float x0[8], x1[8], w[8], wo[8], cs[8], sn[8];
-  unpack_floats(load16(x + 8 * c), x0);
-  unpack_floats(load16(x + 8 * other), x1);
-  unpack_floats(load16(weight + 8 * c), w);
-  unpack_floats(load16(weight + 8 * other), wo);
-  unpack_floats(load16(cos + 8 * (turned ? c : 0)), cs);
-  unpack_floats(load16(sin + 8 * (turned ? c : 0)), sn);
-  F ss = 0, inv;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) ss += (F)(x0[e] * x0[e]);  // x^2 is exact in fp32
-  if constexpr (sizeof(F) == 8) {
-#pragma unroll
-    for (int mask = 1; mask < LPR; mask *= 2) ss += wide_shuffle(ss, mask);
-    const F mean = ss * (F)(1.0 / (8 * LPR)) + (F)eps;
-    inv = (F)rsqrtf((float)mean);
-    // Newton's step on the fp32 root: 2^-22 squares to 2^-44.  Where that root overflows, so does the definition's.
-    inv = mean > (F)0 && isfinite((float)inv) ? inv * (1.5 - 0.5 * mean * inv * inv) : inv;
-  } else {
-    inv = rsqrtf(group_sum<LPR>(ss) * (F)(1.0f / (8 * LPR)) + eps);
+// y_i cos_i - y_{i + R/2} sin_i and the second to y_i cos_i + y_{i - R/2} sin_i, all in F.  The rotation's other half is
+// read from memory again (a line this wave reads anyway) and normalised here, which takes no exchange between lanes.
+template <int LPR>
+struct NormRopeRow {
+  u32x4 x, x_other, w, w_other, cos, sin;
+  bool turned, low;
+  __device__ __forceinline__ void load(const uint16_t *row, const uint16_t *weight, const uint16_t *c, const uint16_t *s,
+                                       int R, int chunk) {
+    const int half = R / 16;  // chunks of half the rotated features
+    low = chunk < half;
+    turned = chunk < 2 * half;
+    const int other = low ? chunk + half : (turned ? chunk - half : chunk);
+    x = load16(row + 8 * chunk);
+    x_other = load16(row + 8 * other);
+    w = load16(weight + 8 * chunk);
+    w_other = load16(weight + 8 * other);
+    cos = load16(c + 8 * (turned ? chunk : 0));
+    sin = load16(s + 8 * (turned ? chunk : 0));
   }
+  static __device__ __forceinline__ double row_sum(double v) {
+    for (int mask = 1; mask < LPR; mask *= 2)
+      v += __hiloint2double(__shfl_xor(__double2hiint(v), mask), __shfl_xor(__double2loint(v), mask));
+    return v;
+  }
+  static __device__ __forceinline__ float row_sum(float v) { return group_sum<LPR>(v); }
+  static __device__ __forceinline__ float root(float v) { return rsqrtf(v); }
+  // Newton's step on the fp32 root: 2^-22 squares to 2^-44.  Where that root is infinite, so is the definition's.
+  static __device__ __forceinline__ double root(double v) {
+    const double r = (double)rsqrtf((float)v);
+    return v > 0 && isfinite((float)r) ? r * (1.5 - 0.5 * v * r * r) : r;
+  }
+  template <typename F>
+  __device__ __forceinline__ void compute(float eps, float offset, float (&y)[8]) const {
+    float a[8], b[8], wa[8], wb[8], cs[8], sn[8];
+    unpack_floats(x, a);
+    unpack_floats(x_other, b);
+    unpack_floats(w, wa);
+    unpack_floats(w_other, wb);
+    unpack_floats(cos, cs);
+    unpack_floats(sin, sn);
+    F ss = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) ss += (F)(a[e] * a[e]);  // x^2 is exact in fp32
+    const F inv = root(row_sum(ss) * (F)(1.0 / (8 * LPR)) + (F)eps);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const F p = (F)a[e] * inv * ((F)wa[e] + (F)offset), q = (F)b[e] * inv * ((F)wb[e] + (F)offset);
+      y[e] = (float)(turned ? p * (F)cs[e] + (low ? -q : q) * (F)sn[e] : p);
+    }
+  }
+};
+
+// Whether a key's codes could be others if its values were off by 2^-20 of the row's largest, which bounds the fp32
+// arithmetic above: a value next to a border of the grid, or a block's largest next to one of the scale.
+template <int LPR>
+__device__ __forceinline__ bool near_border(const float (&y)[8]) {
+  float top = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(y[e]));
+  const uint32_t block = quad_max(__float_as_uint(top));
+  float row = __uint_as_float(block);
+  row = fmaxf(row, dpp_move<kDppHalfMirror>(row));
+  if constexpr (LPR >= 16) row = fmaxf(row, dpp_move<kDppMirror>(row));
+  if constexpr (LPR >= 32) row = pair_max16(row);
+  const float margin = row * 0x1p-20f, largest = __uint_as_float(block);
+  const int scale = kv4_scale(__float_as_uint(largest + margin));
+  float up[8], down[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const F a = (F)x0[e] * inv * ((F)w[e] + (F)offset), b = (F)x1[e] * inv * ((F)wo[e] + (F)offset);
-    y[e] = (float)(turned ? a * (F)cs[e] + (c < half ? -b : b) * (F)sn[e] : a);
+    up[e] = fabsf(y[e]) + margin;
+    down[e] = fmaxf(fabsf(y[e]) - margin, 0.0f);
   }
+  return kv4_scale(__float_as_uint(fmaxf(largest - margin, 0.0f))) != scale ||
+         kv4_codes(up, kv4_scale_value(scale)) != kv4_codes(down, kv4_scale_value(scale));
 }
 
 template <int LPR>
@@ -101,9 +136,12 @@ __global__ void __launch_bounds__(256) norm_rope_kv4_kernel(const Kv4NormRopeArg
   const int heads = query ? a.Hq : Hkv, h = (task - (query ? 0 : q_tasks)) * HEADS + lane / LPR;
   const int hc = min(h, heads - 1);  // lanes past the last head repeat it and write nothing
   const uint16_t *const cos = a.cos.p + b * a.cos.sb + t * a.cos.st, *const sin = a.sin.p + b * a.sin.sb + t * a.sin.st;
+  NormRopeRow<LPR> row;
   float y[8];
   if (query) {
-    norm_rope_row<LPR, float>(a.q.p + b * a.q.sb + hc * a.q.sh + t * a.q.st, a.q_weight, cos, sin, a.eps, a.offset, a.R, c, y);
+    // Rounded once, from fp32 to bf16.
+    row.load(a.q.p + b * a.q.sb + hc * a.q.sh + t * a.q.st, a.q_weight, cos, sin, a.R, c);
+    row.template compute<float>(a.eps, a.offset, y);
     if (h < heads)
       store16(a.q_out + (((int64_t)b * a.Hq + h) * a.T + t) * (8 * LPR) + 8 * c,
               u32x4{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]), pack_bf16x2(y[4], y[5]), pack_bf16x2(y[6], y[7])});
@@ -112,7 +150,16 @@ __global__ void __launch_bounds__(256) norm_rope_kv4_kernel(const Kv4NormRopeArg
     if (!kv4_holds(a.cache, slot)) return;
     float v[8];
     unpack_floats(load16(a.v.p + b * a.v.sb + hc * a.v.sh + t * a.v.st + 8 * c), v);
-    norm_rope_row<LPR, double>(a.k.p + b * a.k.sb + hc * a.k.sh + t * a.k.st, a.k_weight, cos, sin, a.eps, a.offset, a.R, c, y);
+    const uint16_t *key = a.k.p + b * a.k.sb + hc * a.k.sh + t * a.k.st;
+    row.load(key, a.k_weight, cos, sin, a.R, c);
+    row.template compute<float>(a.eps, a.offset, y);
+    // The codes are those of the definition: a wave with a value near a border (under one in a hundred) reads and
+    // computes its rows again in 64 bits.
+    if (__builtin_expect(__any(near_border<LPR>(y)), 0)) {
+      asm volatile("" : "+v"(key));  // not kept in registers for this
+      row.load(key, a.k_weight, cos, sin, a.R, c);
+      row.template compute<double>(a.eps, a.offset, y);
+    }
     kv4_store<LPR>(a.cache, slot, h, c, y, v, h < heads);
   }
 }

@@ -3,7 +3,6 @@
 #include <cmath>
 #include <cstdint>
 #include <limits>
-#include <cstdlib>
 
 #include "xinfer_attention.h"
 #include "kv4_common.h"
@@ -52,28 +51,42 @@ View view_of(const xinfer_view4 &t) {
 }
 
 // Launches and workspace of a paged attention call come from the shapes and the bound on the lengths alone.
-constexpr int kPagedTarget = 512;  // items that fill the chip: two blocks a CU
-constexpr int kPagedDecodeGroups = 16, kPagedPrefillGroups = 8;
+constexpr int kPagedCus = 256;
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-PagedLaunch paged_launch(const PagedArgs &shapes, int vectors_min, int vectors_max, int tile, int min_groups) {
+// Rows may be cut into runs of at least min_groups groups, for about `target` items; whole_groups: rows of no more are not
+// cut, as the merge's launch costs more than it saves.
+PagedLaunch paged_launch(const PagedArgs &shapes, int vectors_min, int vectors_max, int tile, int min_groups, int target,
+                         int whole_groups) {
   PagedLaunch l{shapes, 0, 0, 0};
   l.a.vectors_min = vectors_min;
   l.a.vectors_max = vectors_max;
   l.a.tile = tile;
-  int target = kPagedTarget;
-  if (const char *e = getenv(vectors_max > 32 ? "KV4_PG" : "KV4_DG")) min_groups = atoi(e);
-  if (const char *e = getenv(vectors_max > 32 ? "KV4_PT" : "KV4_DT")) target = atoi(e);
-  l.a.min_groups = min_groups;
   l.a.target = target;
   l.tiles = (int)ceil_div(std::min<int64_t>((int64_t)shapes.T * shapes.G, vectors_max), tile);
   // A row and tile has at most one run more than its share of the target.
-  const int64_t whole = (int64_t)shapes.B * shapes.cache.Hkv * l.tiles;
-  const int64_t runs = ceil_div(ceil_div(shapes.max_length, 64), min_groups);
+  const int64_t whole = (int64_t)shapes.B * shapes.cache.Hkv * l.tiles, groups = ceil_div(shapes.max_length, 64);
+  const int64_t runs = groups <= whole_groups ? 1 : ceil_div(groups, min_groups);
+  l.a.min_groups = runs <= 1 ? (int)std::max<int64_t>(groups, 1) : min_groups;
   l.items = runs <= 1 ? whole : std::min(whole * runs, whole + target);
   l.bytes = runs <= 1 ? 0 : (size_t)l.items * tile * (shapes.cache.D + 2) * sizeof(float);
   return l;
+}
+
+// Decode blocks and items.  One column group: blocks of 4 waves and items enough to fill the chip (16 waves a CU up to
+// 128 features, 8 of 256), since single waves wait for memory and LDS most of the time; runs of two groups a wave, or of
+// one where all those items have a CU of their own.  (8 ragged rows, 128 features: 17.9 us, with 8 waves 19.2; one row
+// of 1024 keys: runs of one group 10.8 us, of two 12.1.)  Two column groups: blocks of 8 waves, one a CU, all at once
+// (six tokens in 8 rows, 32 / 8 heads: 25.4 us, with 4 waves and two blocks a CU 27.5).  In a prefill launch: its
+// blocks' 8 waves.
+PagedLaunch paged_decode_launch(const PagedArgs &shapes, int vectors_max, int tile, bool alone) {
+  const int64_t whole = (int64_t)shapes.B * shapes.cache.Hkv * ceil_div(std::min(shapes.T * shapes.G, vectors_max), tile);
+  const int waves = alone && tile == 16 ? 4 : 8;
+  const int64_t resident = kPagedCus * (waves == 8 ? 1 : shapes.cache.D == 256 ? 2 : 4);
+  const int64_t target = waves == 4 ? resident : std::max(resident - whole, resident / 2);
+  const bool spread = waves == 4 && whole * ceil_div(shapes.max_length, 64 * waves) <= kPagedCus;
+  return paged_launch(shapes, 0, vectors_max, tile, spread ? waves : 8, (int)target, 8);
 }
 
 int paged_call(const xinfer_view4 &q, const xinfer_kv4_cache &cache, int64_t table_width, int64_t max_length,
@@ -94,12 +107,18 @@ int paged_call(const xinfer_view4 &q, const xinfer_kv4_cache &cache, int64_t tab
   a.width = (int32_t)table_width;
   a.max_length = (int32_t)(max_length == 0 ? capacity : std::min(max_length, capacity));
   const int columns = paged_decode_columns(a.cache.D), vectors = a.T * a.G;
-  call.few = paged_launch(a, 0, vectors <= 32 ? 32 : columns, vectors <= 16 ? 16 : columns, kPagedDecodeGroups);
   call.many = PagedLaunch{a, 0, 0, 0};
-  if (vectors > 32) {
-    // One row alone goes to the prefill kernel whatever its count.
-    call.many = paged_launch(a, B == 1 ? 0 : columns + 1, kIntMax, kPagedPrefillTile, kPagedPrefillGroups);
-    if (B == 1) call.few.items = call.few.bytes = 0;
+  if (vectors <= 32) {
+    call.few = paged_decode_launch(a, 32, vectors <= 16 ? 16 : columns, true);
+    return XINFER_OK;
+  }
+  // Rows of more vectors than a decode item has go to the prefill kernel; one row alone does whatever its count.
+  const bool alone = B == 1;
+  call.few = alone ? PagedLaunch{a, 0, 0, 0} : paged_decode_launch(a, columns, columns, false);
+  call.many = paged_launch(a, alone ? 0 : columns + 1, kIntMax, kPagedPrefillTile, 8, alone || B > 64 ? kPagedCus : 3 * kPagedCus, 8);
+  if (!alone) {
+    // A record of 128 vectors is written and read at some 5 TB/s; a group of an item takes about 2 us.
+    if (B <= 64) call.many.a.record_groups = kPagedPrefillTile * 8.0f * (float)a.cache.D / 5e6f / 2.0f;
   }
   return XINFER_OK;
 }

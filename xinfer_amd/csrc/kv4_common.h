@@ -83,6 +83,7 @@ struct PagedArgs {
   // from 0 on, the rows without any too.
   int32_t vectors_min, vectors_max;
   int32_t tile, min_groups, target;
+  float record_groups;  // cost of a record in groups' time; 0: the target as it is (paged_run)
   float *part_o;  // [item][tile][D] unnormalised outputs of rows cut into runs
   float *part_ml;  // [item][tile][2] running maximum (log2 units) and sum
 };
@@ -91,9 +92,9 @@ struct PagedArgs {
 // allow any, to the prefill kernel.
 struct PagedLaunch {
   PagedArgs a;
-  int64_t items;  // blocks; 0: no launch
+  int64_t items;  // of the plan, at most: blocks, and records; 0: no launch
   int tiles;      // of a row and KV head, at most
-  size_t bytes;   // records of rows cut into runs; 0: no row can be
+  size_t bytes;   // of the records; 0: no row can be cut
 };
 struct PagedLaunches {
   PagedLaunch few, many;

@@ -7,24 +7,21 @@
 
 namespace xattn {
 
-template <int D, int NC>
-__global__ void __launch_bounds__(64 * kPagedWaves, D == 256 || NC == 2 ? 2 : 4) paged_decode_kernel(const PagedArgs a) {
-  __shared__ __attribute__((aligned(1024))) char smem[kPagedDecodeLds<D, kPagedWaves>];
-  paged_decode_item<D, NC, kPagedWaves>(a, blockIdx.x, smem);
+// Occupancy: one column group of up to 128 features fits 128 registers (four waves a SIMD), the others twice that.
+template <int D, int NC, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES, D == 256 || NC == 2 ? 2 : 4) paged_decode_kernel(const PagedArgs a) {
+  __shared__ __attribute__((aligned(1024))) char smem[kPagedDecodeLds<D, WAVES>];
+  paged_decode_item<D, NC, WAVES>(a, blockIdx.x, smem);
 }
 
-// Blocks below `few_items` take a decode item, the others a prefill item.
+// Blocks below `few_blocks` take a decode item, the others a prefill item.
 template <int D>
-__global__ void __launch_bounds__(64 * kPagedChunkWaves, 2) paged_both_kernel(const PagedArgs few, const PagedArgs many, int few_items) {
+__global__ void __launch_bounds__(64 * kPagedChunkWaves, 2) paged_both_kernel(const PagedArgs few, const PagedArgs many, int few_blocks) {
   constexpr int WAVES = kPagedChunkWaves, CHUNK = kPagedChunkLds<D>, DECODE = kPagedDecodeLds<D, WAVES>;
   __shared__ __attribute__((aligned(1024))) char smem[CHUNK > DECODE ? CHUNK : DECODE];
-  if ((int)blockIdx.x < few_items) {
-    paged_decode_item<D, paged_decode_columns(D) / 16, WAVES>(few, blockIdx.x, smem);
-  } else if constexpr (D == 256) {
-    paged_chunk_item_wide<D>(many, blockIdx.x - few_items, smem);
-  } else {
-    paged_chunk_item<D>(many, blockIdx.x - few_items, smem);
-  }
+  if ((int)blockIdx.x < few_blocks) paged_decode_item<D, paged_decode_columns(D) / 16, WAVES>(few, blockIdx.x, smem);
+  else if constexpr (D == 256) paged_chunk_item_wide<D>(many, blockIdx.x - few_blocks, smem);
+  else paged_chunk_item<D>(many, blockIdx.x - few_blocks, smem);
 }
 
 // Prefill items alone.
@@ -109,19 +106,23 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedArgs few, c
   }
 }
 
+template <int D, int NC, int WAVES>
+static void launch_decode(const PagedLaunch &l, hipStream_t stream) {
+  hipLaunchKernelGGL((paged_decode_kernel<D, NC, WAVES>), dim3(l.items), dim3(64 * WAVES), 0, stream, l.a);
+}
+
 template <int D>
 static hipError_t launch_d(const PagedLaunches &l, hipStream_t stream) {
-  const dim3 block(64 * kPagedChunkWaves), few_block(64 * kPagedWaves);
+  const dim3 block(64 * kPagedChunkWaves);
   const PagedArgs &few = l.few.a, &many = l.many.a;
   if (l.few.items > 0 && l.many.items > 0) {
     hipLaunchKernelGGL((paged_both_kernel<D>), dim3(l.few.items + l.many.items), block, 0, stream, few, many, (int)l.few.items);
   } else if (l.many.items > 0) {
     hipLaunchKernelGGL((paged_prefill_kernel<D>), dim3(l.many.items), block, 0, stream, many);
   } else if (few.tile == 32) {
-    if constexpr (paged_decode_columns(D) == 32)
-      hipLaunchKernelGGL((paged_decode_kernel<D, 2>), dim3(l.few.items), few_block, 0, stream, few);
+    if constexpr (paged_decode_columns(D) == 32) launch_decode<D, 2, 8>(l.few, stream);
   } else {
-    hipLaunchKernelGGL((paged_decode_kernel<D, 1>), dim3(l.few.items), few_block, 0, stream, few);
+    launch_decode<D, 1, 4>(l.few, stream);
   }
   if (l.bytes() > 0) {
     constexpr int VECTORS = 256 / (D / 4) * kMergeVectors;

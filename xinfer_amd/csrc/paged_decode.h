@@ -20,7 +20,6 @@
 
 namespace xattn {
 
-constexpr int kPagedWaves = 4;  // of a decode block
 constexpr float kLowest = -3.0e38f;  // running maximum before any key
 
 template <int D>

@@ -2,8 +2,8 @@
 //
 // A launch is sized by the shapes alone.  Its waves each compute the same plan from the lengths: a row's keys are
 // cut into `nsplit` runs of 64-key groups, its query vectors (query heads of a KV head times tokens) into tiles, and
-// an item is a (tile, run, KV head).  Runs take at least `min_groups` groups, and as many more as leave about
-// `target` items, so a few long rows fill the chip and many rows are not cut at all.  Items past the plan's last end
+// an item is a (tile, run, KV head).  Runs take at least `min_groups` groups, and as many more as leave at most about
+// `target` items (paged_run), so a few long rows fill the chip and many rows are not cut at all.  Items past the plan's last end
 // at once.  The KV head counts fastest: consecutive blocks go to the 8 XCDs in turn, so with 8 KV heads the tiles
 // of one head meet in one XCD's L2.
 #pragma once
@@ -62,7 +62,19 @@ struct PagedRows {
   }
 };
 
+__device__ __forceinline__ int paged_splits(const PagedShare &s, int run) { return max(1, (s.groups + run - 1) / run); }
+
 // Groups of a run at most.
+//
+// Prefill items of ragged batches are long and of different lengths, so what a target of items gives is estimated for
+// eight: n items of at most m groups on kPagedSlots blocks at a time take no longer than ceil(n / slots) m, nor than
+// their mean load and m; an item costs kPagedItemGroups more (queries in, output out) and a record what it is written
+// and read for (a.record_groups).  On a batch of 5 rows of 33 to 223 groups, 256 features: 434 us with the target so
+// found (768), 500 with 512, 515 with 256; on uniform batches 256 is best (4 rows of 64 groups, 128 features: 88 us, 117
+// with 768).
+constexpr int kPagedSlots = 256;
+constexpr float kPagedItemGroups = 4.0f;
+
 __device__ __forceinline__ int paged_run(const PagedArgs &a, const PagedRows &first) {
   float total = (float)first.s.groups * (float)first.s.tiles;
   for (int base = 64; base < a.B; base += 64) {
@@ -71,9 +83,28 @@ __device__ __forceinline__ int paged_run(const PagedArgs &a, const PagedRows &fi
     total += (float)rows.s.groups * (float)rows.s.tiles;
   }
   total = group_sum<64>(total) * (float)a.cache.Hkv;
-  return max(a.min_groups, (int)(total / (float)a.target) + 1);
+  if (a.record_groups <= 0.0f) return max(a.min_groups, (int)(total / (float)a.target) + 1);
+  // Eight targets at a time, each by eight lanes, which take every eighth row.
+  const int lane = threadIdx.x & 63, target = min(kPagedSlots + kPagedSlots / 4 * (lane >> 3), a.target);
+  const int run = max(a.min_groups, (int)(total / (float)target) + 1);
+  float n = 0.0f, records = 0.0f, longest = 0.0f;
+  for (int base = 0; base < a.B; base += 8) {
+    const int from = base + (lane & 7), groups = __shfl(first.s.groups, from), tiles = __shfl(first.s.tiles, from);
+    const int nsplit = max(1, (groups + run - 1) / run);
+    const float items = (float)(tiles * nsplit);
+    n += items;
+    records += nsplit > 1 ? items : 0.0f;
+    longest = fmaxf(longest, (float)((groups + nsplit - 1) / nsplit));
+  }
+  n = group_sum<8>(n) * (float)a.cache.Hkv;
+  records = group_sum<8>(records) * (float)a.cache.Hkv;
+  for (int mask = 1; mask < 8; mask *= 2) longest = fmaxf(longest, __shfl_xor(longest, mask));
+  const float m = longest + kPagedItemGroups, rounds = ceilf(n / (float)kPagedSlots) * m;
+  const float cost = fminf(rounds, (total + n * kPagedItemGroups) / (float)kPagedSlots + m) + records * a.record_groups;
+  float best = cost;
+  for (int mask = 8; mask < 64; mask *= 2) best = fminf(best, __shfl_xor(best, mask));
+  return __builtin_amdgcn_readlane(run, __builtin_ctzll(__ballot(cost == best)));
 }
-__device__ __forceinline__ int paged_splits(const PagedShare &s, int run) { return max(1, (s.groups + run - 1) / run); }
 
 // What lane `at` holds of its row; upto: items up to and with it.
 __device__ __forceinline__ void paged_take(PagedItem &it, const PagedRows &rows, int nsplit, int upto, int items, int at) {
