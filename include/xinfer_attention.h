@@ -256,7 +256,7 @@ typedef struct xinfer_kv4_cache {
  * ring's head and tail; it must not be counters.  The same inputs give the same
  * results again.  Out-of-range lengths are clamped ([0, tokens] new tokens,
  * lengths of at least that), so no input reaches outside the arrays.
- * table_width * page_size and rows * table_width stay below 2^31. */
+ * table_width * page_size is at most 2^30, rows * table_width below 2^31. */
 int xinfer_paged_kv_reserve(const int32_t *kv_before, const int32_t *kv_lengths, const int32_t *query_lengths,
                             int64_t rows, int64_t tokens, int64_t page_size, const int64_t *counters,
                             int32_t *block_table, int64_t table_width, int32_t *free_pages, int64_t ring_size,

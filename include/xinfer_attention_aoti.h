@@ -75,6 +75,33 @@ AOTITorchError aoti_torch_cuda_qk_norm_rope_append(
 AOTITorchError aoti_torch_cuda_projection_gemv(AtenTensorHandle x, AtenTensorHandle weight,
                                                AtenTensorHandle *output);
 
+/* The paged 4-bit KV cache's operators (xinfer_attention.h; no reference
+ * counterpart): pages, slots and positions; append; read-back; q/k norm, rotation
+ * and append; attention.  The caches, the page table and the ring of free pages
+ * change in place; the append's output slot is never written. */
+AOTITorchError aoti_torch_cuda_paged_kv_reserve(
+    AtenTensorHandle kv_before, AtenTensorHandle kv_lengths, AtenTensorHandle query_lengths, int64_t tokens,
+    int64_t page_size, AtenTensorHandle counters, AtenTensorHandle block_table, AtenTensorHandle free_pages,
+    AtenTensorHandle *lengths, AtenTensorHandle *positions, AtenTensorHandle *slots,
+    AtenTensorHandle *new_counters);
+AOTITorchError aoti_torch_cuda_append_kv4(AtenTensorHandle key, AtenTensorHandle value, AtenTensorHandle slots,
+                                          AtenTensorHandle key_codes, AtenTensorHandle key_scales,
+                                          AtenTensorHandle value_codes, AtenTensorHandle value_scales,
+                                          AtenTensorHandle *unused_output);
+AOTITorchError aoti_torch_cuda_read_kv4(AtenTensorHandle key_codes, AtenTensorHandle key_scales,
+                                        AtenTensorHandle value_codes, AtenTensorHandle value_scales,
+                                        AtenTensorHandle slots, AtenTensorHandle *key, AtenTensorHandle *value);
+AOTITorchError aoti_torch_cuda_qk_norm_rope_append_kv4(
+    AtenTensorHandle q, AtenTensorHandle key, AtenTensorHandle value, AtenTensorHandle q_weight,
+    AtenTensorHandle k_weight, double eps, double weight_offset, AtenTensorHandle cos, AtenTensorHandle sin,
+    AtenTensorHandle slots, AtenTensorHandle key_codes, AtenTensorHandle key_scales,
+    AtenTensorHandle value_codes, AtenTensorHandle value_scales, AtenTensorHandle *output);
+AOTITorchError aoti_torch_cuda_paged_attention_kv4(AtenTensorHandle q, AtenTensorHandle key_codes,
+                                                   AtenTensorHandle key_scales, AtenTensorHandle value_codes,
+                                                   AtenTensorHandle value_scales, AtenTensorHandle block_table,
+                                                   AtenTensorHandle lengths, int64_t max_length, double scale,
+                                                   AtenTensorHandle *output);
+
 #ifdef __cplusplus
 }
 #endif

@@ -21,6 +21,12 @@ embedding and append in one native launch) followed by
 ``batched_flash_attention_bthd``, whose [B, T, Hq, D] output makes the
 reshape before o_proj a view.
 
+Both families also run over a paged cache held in 4 bits (paged_kv4.py): ``PagedStep``,
+``Qwen3PagedAttention``, ``Qwen35PagedAttention`` and ``PagedModelStep``.  A
+step builds its page tables and slots on the device, each layer is one
+``qk_norm_rope_append_kv4`` and one ``paged_attention_kv4``, and nothing reads a
+length on the host, so a step can be captured in a HIP graph as it is.
+
 The adapters reject what the native path does not implement, with ValueError
 as the reference's adapters do: training mode, returned attention weights, an
 explicit attention mask (causality comes from the cache lengths), a cache that
@@ -32,6 +38,8 @@ from __future__ import annotations
 import torch
 
 from .attention import batched_attention_metadata, load_attention_ops, require
+from .paged_kv4 import (HEAD_DIMS, append_kv4, paged_attention_kv4, paged_kv4_cache, paged_kv_reserve,
+                        qk_norm_rope_append_kv4)
 
 # Export bounds of the model steps (compiler/qwen35/config.py:8-9): batch and
 # prefill tokens per step.
@@ -76,17 +84,18 @@ def _check_geometry(module):
     require(8 <= dim <= 256 and dim % 8 == 0, "Flash head dimension must be a multiple of 8 in 8..256")
 
 
-def _step_cache(adapter, attention_mask, kwargs):
-    """The call's KVCache, after the checks every adapter makes."""
+def _step_cache(adapter, attention_mask, kwargs, kind=KVCache):
+    """The call's KVCache (or PagedStep), after the checks every adapter makes."""
     require(not adapter.training and not kwargs.get("output_attentions", False),
             "Flash adapter supports inference without attention weights")
     require(attention_mask is None, "Flash adapter uses KVCache lengths instead of attention masks")
     cache = kwargs.get("past_key_values")
     if cache is None:
         cache = kwargs.get("past_key_value")
-    require(isinstance(cache, KVCache), "Flash adapter requires a KVCache with per-row lengths")
+    require(isinstance(cache, kind), f"Flash adapter requires a {kind.__name__} with per-row lengths")
     position = kwargs.get("cache_position")
-    require(position is None or position is cache.position, "Flash adapter requires KVCache with the same position tensor")
+    require(position is None or position is cache.position,
+            f"Flash adapter requires {kind.__name__} with the same position tensor")
     return cache
 
 
@@ -179,6 +188,93 @@ class Qwen35FlashAttention(torch.nn.Module):
         return a.o_proj(out * torch.sigmoid(gate)), None
 
 
+class PagedStep:
+    """Paged 4-bit caches of one step, with its positions, slots and lengths.
+
+    ``tensors[4 * i : 4 * i + 4]`` are layer i's cache (paged_kv4.paged_kv4_cache); ``lengths`` int32 [2, B],
+    ``position`` and ``slots`` int64 [B, T] come from ``paged_kv_reserve``, ``block_table`` int32 [B, M] from the serving
+    loop; ``max_length`` is its bound on the rows' lengths (0: what the table can hold).  Built once per step and shared
+    by every layer.
+    """
+
+    def __init__(self, tensors, position, slots, lengths, block_table, max_length=0):
+        self.tensors = tuple(tensors)
+        self.position, self.slots, self.lengths = position, slots, lengths
+        self.block_table, self.max_length = block_table, max_length
+
+    def layer(self, index):
+        return self.tensors[4 * index : 4 * index + 4]
+
+    def update(self, key, value, layer_idx, cache_kwargs=None):
+        """Append key/value [B, Hkv, T, D] at the step's slots (real tokens only); returns the layer's cache."""
+        cache = self.layer(layer_idx)
+        append_kv4(key, value, self.slots, cache)
+        return cache
+
+
+def _check_paged_geometry(module):
+    _check_geometry(module)
+    require(module.head_dim in HEAD_DIMS, f"The 4-bit cache holds head dimensions {HEAD_DIMS}")
+
+
+class Qwen3PagedAttention(torch.nn.Module):
+    """Qwen3Attention's weights around the paged 4-bit operators."""
+
+    def __init__(self, original):
+        super().__init__()
+        from transformers.models.qwen3.modeling_qwen3 import Qwen3Attention
+
+        require(type(original) is Qwen3Attention and original.sliding_window is None,
+                "Expected full-attention Qwen3Attention")
+        _check_paged_geometry(original)
+        require(original.q_norm.variance_epsilon == original.k_norm.variance_epsilon,
+                "The fused norm/rope step needs one RMSNorm epsilon for q and k")
+        self.original = original
+
+    def forward(self, hidden_states, position_embeddings, attention_mask=None, **kwargs):
+        step = _step_cache(self, attention_mask, kwargs, PagedStep)
+        a = self.original
+        batch_shape = hidden_states.shape[:-1]
+        per_head = (*batch_shape, -1, a.head_dim)
+        cos, sin = position_embeddings
+        cache = step.layer(a.layer_idx)
+        q = qk_norm_rope_append_kv4(a.q_proj(hidden_states).view(per_head), a.k_proj(hidden_states).view(per_head),
+                                    a.v_proj(hidden_states).view(per_head), a.q_norm.weight, a.k_norm.weight,
+                                    a.q_norm.variance_epsilon, 0.0, cos, sin, step.slots, cache)
+        out = paged_attention_kv4(q, cache, step.block_table, step.lengths, step.max_length, a.scaling)
+        return a.o_proj(out.reshape(*batch_shape, -1)), None
+
+
+class Qwen35PagedAttention(torch.nn.Module):
+    """Qwen3.5's gated full attention around the paged 4-bit operators.
+
+    Its RMSNorm weights are stored minus one, its rotary embedding turns the first rotary_dim features of a head, and
+    the query is half of what q_proj yields; the norm/rope step takes all three as they are.
+    """
+
+    def __init__(self, original):
+        super().__init__()
+        from transformers.models.qwen3_5.modeling_qwen3_5 import Qwen3_5Attention
+
+        require(type(original) is Qwen3_5Attention, "Expected Qwen3.5 full attention")
+        _check_paged_geometry(original)
+        self.original = original
+
+    def forward(self, hidden_states, position_embeddings, attention_mask=None, **kwargs):
+        step = _step_cache(self, attention_mask, kwargs, PagedStep)
+        a = self.original
+        batch_shape = hidden_states.shape[:-1]
+        per_head = (*batch_shape, -1, a.head_dim)
+        query, gate = torch.chunk(a.q_proj(hidden_states).view(*batch_shape, -1, 2 * a.head_dim), 2, dim=-1)
+        cos, sin = position_embeddings
+        cache = step.layer(a.layer_idx)
+        q = qk_norm_rope_append_kv4(query, a.k_proj(hidden_states).view(per_head), a.v_proj(hidden_states).view(per_head),
+                                    a.q_norm.weight, a.k_norm.weight, a.config.rms_norm_eps, 1.0, cos, sin, step.slots,
+                                    cache)
+        out = paged_attention_kv4(q, cache, step.block_table, step.lengths, step.max_length, a.scaling)
+        return a.o_proj(out.reshape(*batch_shape, -1) * torch.sigmoid(gate.reshape(*batch_shape, -1))), None
+
+
 def model_family(model):
     """'qwen3' or 'qwen35' from the model's configuration type."""
     model_type = model.config.model_type
@@ -207,6 +303,29 @@ def install_attention(model, *, fused=False):
             continue
         adapter = Qwen3FlashAttention(layer.self_attn, fused=fused) if family == "qwen3" else \
             Qwen35FlashAttention(layer.self_attn)
+        adapter.train(layer.self_attn.training)
+        replacements.append((layer, adapter))
+    load_attention_ops(model=family)
+    for layer, adapter in replacements:
+        layer.self_attn = adapter
+    return model
+
+
+def install_paged_attention(model):
+    """Replace each attention module of ``model`` by its paged 4-bit adapter, keeping the original weights.
+
+    As ``install_attention``: every replacement is built (and checked) before any layer changes.
+    """
+    family = model_family(model)
+    if family == "qwen35":
+        require(all(kind == "full_attention" for kind in model.config.layer_types),
+                "Linear-attention layers are not attention operators of this library")
+    kind = Qwen3PagedAttention if family == "qwen3" else Qwen35PagedAttention
+    replacements = []
+    for layer in model.model.layers:
+        if isinstance(layer.self_attn, kind):
+            continue
+        adapter = kind(layer.self_attn)
         adapter.train(layer.self_attn.training)
         replacements.append((layer, adapter))
     load_attention_ops(model=family)
@@ -271,3 +390,46 @@ class ModelStep(torch.nn.Module):
         last = hidden.gather(1, (counts - 1).clamp_min(0)[:, None, None].expand(-1, 1, hidden.shape[-1]))
         logits = self.model.lm_head(last)[:, 0, :]
         return logits.masked_fill(counts[:, None] == 0, 0)
+
+
+class PagedModelStep(torch.nn.Module):
+    """One inference step of a causal LM over paged 4-bit caches, without a length on the host.
+
+    forward(input_ids [B, T] int64, kv_before, kv_lengths and query_lengths int32 [B] on the device, kv (4 tensors per
+    layer, ``cache``), counters, block_table, free_pages, max_length) -> (logits [B, vocab] of each row's last real
+    token, lengths [2, B], counters).  The pages are reserved first (``paged_kv_reserve``: kv_before is each row's
+    length before the step, kv_lengths after it); a row without pages to be had takes no part, its count in
+    ``lengths`` is 0 and its logits are zero, as those of rows without new tokens.  block_table, free_pages and the caches
+    change in place; the next step's kv_before is lengths[1], its counters the returned ones.
+    """
+
+    def __init__(self, model):
+        super().__init__()
+        install_paged_attention(model)
+        self.model = model
+        self.eval()
+
+    def cache(self, pages, page_size, device="cuda"):
+        """Empty caches of every layer, 4 tensors each."""
+        config = self.model.config
+        head_dim = self.model.model.layers[0].self_attn.original.head_dim
+        return tuple(t for _ in self.model.model.layers
+                     for t in paged_kv4_cache(pages, config.num_key_value_heads, page_size, head_dim, device))
+
+    def forward(self, input_ids, kv_before, kv_lengths, query_lengths, kv, counters, block_table, free_pages,
+                max_length=0):
+        lengths, positions, slots, counters = paged_kv_reserve(
+            kv_before, kv_lengths, query_lengths, input_ids.shape[1], kv[0].shape[2], counters, block_table, free_pages)
+        step = PagedStep(kv, positions, slots, lengths, block_table, max_length)
+        base = self.model.model
+        hidden = base.embed_tokens(input_ids)
+        rotary = rotary_tables(self.model, hidden, positions)
+        for layer in base.layers:
+            out = layer(hidden, attention_mask=None, position_ids=positions, past_key_values=step,
+                        cache_position=positions, position_embeddings=rotary, use_cache=True)
+            hidden = out[0] if isinstance(out, tuple) else out
+        hidden = base.norm(hidden)
+        counts = lengths[0].to(torch.int64)
+        last = hidden.gather(1, (counts - 1).clamp_min(0)[:, None, None].expand(-1, 1, hidden.shape[-1]))
+        logits = self.model.lm_head(last)[:, 0, :]
+        return logits.masked_fill(counts[:, None] == 0, 0), lengths, counters

@@ -1029,7 +1029,8 @@ const char *xinfer_status_string(int status) {
              "aligned data";
     case XINFER_ERR_KV4_SHAPE: return "Tensors do not match the 4-bit KV cache or each other";
     case XINFER_ERR_PAGES:
-      return "Expected pages of 64, 128 or 256 tokens, and a page table and a ring of free pages below 2^31 entries";
+      return "Expected pages of 64, 128 or 256 tokens, a page table of at most 2^30 tokens a row and 2^31 entries, and a "
+             "ring of free pages";
     default: return "Unknown xinfer status";
   }
 }

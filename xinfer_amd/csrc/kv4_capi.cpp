@@ -12,6 +12,7 @@ namespace xattn {
 namespace {
 
 constexpr int64_t kIntMax = std::numeric_limits<int32_t>::max();
+constexpr int64_t kMostTokens = int64_t(1) << 30;  // of a page table's row: positions stay in 32 bits
 
 bool aligned16(const void *p) { return p != nullptr && (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
@@ -96,7 +97,7 @@ int paged_call(const xinfer_view4 &q, const xinfer_kv4_cache &cache, int64_t tab
   const int64_t B = q.size[0], Hq = q.size[1], T = q.size[2];
   if (B < 0 || B > 65535 || T < 0 || q.size[3] != a.cache.D) return XINFER_ERR_KV4_SHAPE;
   if (Hq < 1 || Hq > 65535 || Hq % a.cache.Hkv != 0) return XINFER_ERR_HEADS;
-  if (table_width < 1 || table_width > kIntMax >> a.cache.page_shift || max_length < 0) return XINFER_ERR_PAGES;
+  if (table_width < 1 || table_width > kMostTokens >> a.cache.page_shift || max_length < 0) return XINFER_ERR_PAGES;
   // Query vectors and items are counted in 32 bits.
   if (T > (kIntMax >> 8) / Hq || B * Hq * T > kIntMax >> 4) return XINFER_ERR_KV4_SHAPE;
   const int64_t capacity = table_width << a.cache.page_shift;
@@ -138,7 +139,7 @@ int xinfer_paged_kv_reserve(const int32_t *kv_before, const int32_t *kv_lengths,
                             int32_t *lengths, int64_t *positions, int64_t *slots, int64_t *new_counters,
                             void *stream) {
   const int shift = page_shift(page_size);
-  if (shift < 0 || table_width < 1 || table_width > kIntMax >> shift || ring_size < 1 || ring_size > kIntMax)
+  if (shift < 0 || table_width < 1 || table_width > kMostTokens >> shift || ring_size < 1 || ring_size > kIntMax)
     return XINFER_ERR_PAGES;
   if (rows < 0 || tokens < 0 || tokens > kIntMax) return XINFER_ERR_ARGUMENT;
   if (rows > kIntMax / table_width) return XINFER_ERR_PAGES;

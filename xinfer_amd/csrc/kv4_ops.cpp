@@ -227,3 +227,79 @@ TORCH_LIBRARY_IMPL(xinfer, CUDA, m) {
   m.impl("qk_norm_rope_append_kv4", TORCH_FN(xinfer::qk_norm_rope_append_kv4));
   m.impl("paged_attention_kv4", TORCH_FN(xinfer::paged_attention_kv4));
 }
+
+using torch::aot_inductor::new_tensor_handle;
+using torch::aot_inductor::resolve_tensor_dispatch_flags;
+
+extern "C" {
+
+AOTI_TORCH_EXPORT AOTITorchError aoti_torch_cuda_paged_kv_reserve(
+    AtenTensorHandle kv_before, AtenTensorHandle kv_lengths, AtenTensorHandle query_lengths, int64_t tokens,
+    int64_t page_size, AtenTensorHandle counters, AtenTensorHandle block_table, AtenTensorHandle free_pages,
+    AtenTensorHandle *lengths, AtenTensorHandle *positions, AtenTensorHandle *slots, AtenTensorHandle *new_counters) {
+  AOTI_TORCH_CONVERT_EXCEPTION_TO_ERROR_CODE({
+    auto [l, p, s, c] = xinfer::paged_kv_reserve(
+        resolve_tensor_dispatch_flags(kv_before), resolve_tensor_dispatch_flags(kv_lengths),
+        resolve_tensor_dispatch_flags(query_lengths), tokens, page_size, resolve_tensor_dispatch_flags(counters),
+        resolve_tensor_dispatch_flags(block_table), resolve_tensor_dispatch_flags(free_pages));
+    *lengths = new_tensor_handle(std::move(l));
+    *positions = new_tensor_handle(std::move(p));
+    *slots = new_tensor_handle(std::move(s));
+    *new_counters = new_tensor_handle(std::move(c));
+  });
+}
+
+AOTI_TORCH_EXPORT AOTITorchError aoti_torch_cuda_append_kv4(
+    AtenTensorHandle key, AtenTensorHandle value, AtenTensorHandle slots, AtenTensorHandle key_codes,
+    AtenTensorHandle key_scales, AtenTensorHandle value_codes, AtenTensorHandle value_scales,
+    AtenTensorHandle * /*unused_output*/) {
+  AOTI_TORCH_CONVERT_EXCEPTION_TO_ERROR_CODE({
+    xinfer::append_kv4(resolve_tensor_dispatch_flags(key), resolve_tensor_dispatch_flags(value),
+                       resolve_tensor_dispatch_flags(slots), resolve_tensor_dispatch_flags(key_codes),
+                       resolve_tensor_dispatch_flags(key_scales), resolve_tensor_dispatch_flags(value_codes),
+                       resolve_tensor_dispatch_flags(value_scales));
+  });
+}
+
+AOTI_TORCH_EXPORT AOTITorchError aoti_torch_cuda_read_kv4(AtenTensorHandle key_codes, AtenTensorHandle key_scales,
+                                                          AtenTensorHandle value_codes, AtenTensorHandle value_scales,
+                                                          AtenTensorHandle slots, AtenTensorHandle *key,
+                                                          AtenTensorHandle *value) {
+  AOTI_TORCH_CONVERT_EXCEPTION_TO_ERROR_CODE({
+    auto [k, v] = xinfer::read_kv4(resolve_tensor_dispatch_flags(key_codes), resolve_tensor_dispatch_flags(key_scales),
+                                   resolve_tensor_dispatch_flags(value_codes),
+                                   resolve_tensor_dispatch_flags(value_scales), resolve_tensor_dispatch_flags(slots));
+    *key = new_tensor_handle(std::move(k));
+    *value = new_tensor_handle(std::move(v));
+  });
+}
+
+AOTI_TORCH_EXPORT AOTITorchError aoti_torch_cuda_qk_norm_rope_append_kv4(
+    AtenTensorHandle q, AtenTensorHandle key, AtenTensorHandle value, AtenTensorHandle q_weight,
+    AtenTensorHandle k_weight, double eps, double weight_offset, AtenTensorHandle cos, AtenTensorHandle sin,
+    AtenTensorHandle slots, AtenTensorHandle key_codes, AtenTensorHandle key_scales, AtenTensorHandle value_codes,
+    AtenTensorHandle value_scales, AtenTensorHandle *output) {
+  AOTI_TORCH_CONVERT_EXCEPTION_TO_ERROR_CODE({
+    *output = new_tensor_handle(xinfer::qk_norm_rope_append_kv4(
+        resolve_tensor_dispatch_flags(q), resolve_tensor_dispatch_flags(key), resolve_tensor_dispatch_flags(value),
+        resolve_tensor_dispatch_flags(q_weight), resolve_tensor_dispatch_flags(k_weight), eps, weight_offset,
+        resolve_tensor_dispatch_flags(cos), resolve_tensor_dispatch_flags(sin), resolve_tensor_dispatch_flags(slots),
+        resolve_tensor_dispatch_flags(key_codes), resolve_tensor_dispatch_flags(key_scales),
+        resolve_tensor_dispatch_flags(value_codes), resolve_tensor_dispatch_flags(value_scales)));
+  });
+}
+
+AOTI_TORCH_EXPORT AOTITorchError aoti_torch_cuda_paged_attention_kv4(
+    AtenTensorHandle q, AtenTensorHandle key_codes, AtenTensorHandle key_scales, AtenTensorHandle value_codes,
+    AtenTensorHandle value_scales, AtenTensorHandle block_table, AtenTensorHandle lengths, int64_t max_length, double scale,
+    AtenTensorHandle *output) {
+  AOTI_TORCH_CONVERT_EXCEPTION_TO_ERROR_CODE({
+    *output = new_tensor_handle(xinfer::paged_attention_kv4(
+        resolve_tensor_dispatch_flags(q), resolve_tensor_dispatch_flags(key_codes),
+        resolve_tensor_dispatch_flags(key_scales), resolve_tensor_dispatch_flags(value_codes),
+        resolve_tensor_dispatch_flags(value_scales), resolve_tensor_dispatch_flags(block_table),
+        resolve_tensor_dispatch_flags(lengths), max_length, scale));
+  });
+}
+
+}  // extern "C"

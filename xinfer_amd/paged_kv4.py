@@ -24,7 +24,36 @@ PAGE_SIZES = (64, 128, 256)
 HEAD_DIMS = (64, 128, 256)
 
 
+# AOTInductor C-shim declarations (include/xinfer_attention_aoti.h).
+_CACHE_SHIM = """AtenTensorHandle key_codes, AtenTensorHandle key_scales,
+    AtenTensorHandle value_codes, AtenTensorHandle value_scales"""
+PAGED_C_SHIMS = {
+    "paged_kv_reserve": """AOTITorchError aoti_torch_cuda_paged_kv_reserve(
+    AtenTensorHandle kv_before, AtenTensorHandle kv_lengths, AtenTensorHandle query_lengths, int64_t tokens,
+    int64_t page_size, AtenTensorHandle counters, AtenTensorHandle block_table, AtenTensorHandle free_pages,
+    AtenTensorHandle* lengths, AtenTensorHandle* positions, AtenTensorHandle* slots,
+    AtenTensorHandle* new_counters)""",
+    "append_kv4": f"""AOTITorchError aoti_torch_cuda_append_kv4(
+    AtenTensorHandle key, AtenTensorHandle value, AtenTensorHandle slots, {_CACHE_SHIM},
+    AtenTensorHandle* unused_output)""",
+    "read_kv4": f"""AOTITorchError aoti_torch_cuda_read_kv4(
+    {_CACHE_SHIM}, AtenTensorHandle slots, AtenTensorHandle* key, AtenTensorHandle* value)""",
+    "qk_norm_rope_append_kv4": f"""AOTITorchError aoti_torch_cuda_qk_norm_rope_append_kv4(
+    AtenTensorHandle q, AtenTensorHandle key, AtenTensorHandle value, AtenTensorHandle q_weight,
+    AtenTensorHandle k_weight, double eps, double weight_offset, AtenTensorHandle cos, AtenTensorHandle sin,
+    AtenTensorHandle slots, {_CACHE_SHIM}, AtenTensorHandle* output)""",
+    "paged_attention_kv4": f"""AOTITorchError aoti_torch_cuda_paged_attention_kv4(
+    AtenTensorHandle q, {_CACHE_SHIM}, AtenTensorHandle block_table, AtenTensorHandle lengths, int64_t max_length,
+    double scale, AtenTensorHandle* output)""",
+}
 _calls = {}
+
+
+def paged_c_shims():
+    """Inductor's call declarations for the paged operators, to go with ``attention_c_shims()``."""
+    return {_call(name): [text] for name, text in PAGED_C_SHIMS.items()}
+
+
 
 
 def _call(name):
