@@ -256,7 +256,8 @@ typedef struct xinfer_kv4_cache {
  * ring's head and tail; it must not be counters.  The same inputs give the same
  * results again.  Out-of-range lengths are clamped ([0, tokens] new tokens,
  * lengths of at least that), so no input reaches outside the arrays.
- * table_width * page_size is at most 2^30, rows * table_width below 2^31. */
+ * table_width * page_size is at most 2^30, rows at most 65535, rows * table_width
+ * below 2^31. */
 int xinfer_paged_kv_reserve(const int32_t *kv_before, const int32_t *kv_lengths, const int32_t *query_lengths,
                             int64_t rows, int64_t tokens, int64_t page_size, const int64_t *counters,
                             int32_t *block_table, int64_t table_width, int32_t *free_pages, int64_t ring_size,
@@ -266,7 +267,7 @@ int xinfer_paged_kv_reserve(const int32_t *kv_before, const int32_t *kv_lengths,
 /* Quantises key/value [B,Hkv,T,D] (bf16, layout as for attention tensors) into
  * slots [B,T] (device int64, strides in elements).  Slots outside the cache,
  * negative ones among them, are skipped.  The slots of one call are distinct; one
- * given twice holds codes of either token. */
+ * given twice holds a mixture of its tokens. */
 int xinfer_append_kv4(const xinfer_view4 *key, const xinfer_view4 *value, const int64_t *slots,
                       int64_t slot_stride_b, int64_t slot_stride_t, const xinfer_kv4_cache *cache, void *stream);
 
@@ -280,9 +281,10 @@ int xinfer_read_kv4(const xinfer_kv4_cache *cache, const int64_t *slots, int64_t
  * row: y = x * rsqrt(mean(x^2) + eps) * (weight + weight_offset), then the first
  * R features turn by cos/sin [B,1,T,R] (R = cos->size[3], a multiple of 16 up to D):
  * y_i cos_i - y_{i+R/2} sin_i for i < R/2, y_i cos_i + y_{i-R/2} sin_i for the
- * second half.  All in fp32; the query is rounded once into q_out, contiguous
- * [B,Hq,T,D], for every token; the key is quantised from fp32 and appended with the
- * value as in xinfer_append_kv4.  weight_offset: 0, or 1 for weights stored minus
+ * second half.  The query is computed in fp32 and rounded once into q_out, contiguous
+ * [B,Hq,T,D], for every token; the key is quantised without a rounding in front
+ * (where fp32 could decide a code, in 64 bits) and appended with the value as in
+ * xinfer_append_kv4.  weight_offset: 0, or 1 for weights stored minus
  * one. */
 int xinfer_qk_norm_rope_append_kv4(const xinfer_view4 *q, const xinfer_view4 *key, const xinfer_view4 *value,
                                    const void *q_weight, const void *k_weight, double eps, double weight_offset,

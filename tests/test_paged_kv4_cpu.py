@@ -60,6 +60,7 @@ def test_reserve_refusals(lib):
     assert call(size=32) == call(size=96) == call(size=512) == call(size=0) == PAGES
     assert call(width=0) == call(width=(1 << 24) + 1) == call(ring=0) == call(ring=1 << 31) == PAGES
     assert call(rows=1 << 29) == PAGES
+    assert call(rows=65536, width=1) == ARGUMENT
     assert call(rows=-1) == call(tokens=-1) == call(pointer=0) == call(counters=0) == call(after=BASE) == ARGUMENT
 
 
@@ -72,6 +73,8 @@ def test_append_and_read_refusals(lib):
         assert lib.xinfer_read_kv4(held, PTR(BASE), I64(3), I64(1), I64(2), I64(3), PTR(BASE), PTR(BASE), None) == CACHE
     assert append(key=view(2, 4, 3, 128)) == append(value=view(2, 8, 4, 128)) == append(key=view(2, 8, 3, 64)) == SHAPE
     assert append(view(1 << 20, 8, 1 << 20, 128), view(1 << 20, 8, 1 << 20, 128)) == SHAPE
+    # A launch's threads are counted in 32 bits: 16 for each of 2^28 rows.
+    assert append(view(1 << 12, 8, 1 << 13, 128), view(1 << 12, 8, 1 << 13, 128)) == SHAPE
     assert append(slots=0) == append(key=None) == append(held=None) == ARGUMENT
     odd = view(2, 8, 3, 128, strides=[8 * 3 * 132, 3 * 132, 132, 1])
     assert append(odd) == append(view(2, 8, 3, 128, data=BASE + 2)) == append(view(2, 8, 3, 128, strides=[9, 9, 9, 2])) == LAYOUT
@@ -94,6 +97,8 @@ def test_norm_rope_refusals(lib):
         assert call(rope=view(2, 1, 3, width)) == SHAPE
     assert call(rope=view(2, 2, 3, 128)) == call(rope=view(2, 1, 4, 128)) == SHAPE
     assert call(eps=-1.0) == call(eps=float("nan")) == EPS
+    wide = [view(1 << 12, heads, 1 << 13, 128) for heads in (1, 8)]
+    assert call(q=wide[0], key=wide[1], rope=view(1 << 12, 1, 1 << 13, 128)) == SHAPE
     assert call(offset=float("inf")) == call(slots=0) == call(weight=0) == ARGUMENT
     assert call(weight=BASE + 2) == call(q=view(2, 16, 3, 128, data=BASE + 4)) == LAYOUT
 
@@ -105,6 +110,7 @@ def test_attention_refusals_and_workspace(lib):
 
     assert call(held=cache(page_size=16)) == CACHE
     assert call(view(2, 16, 1, 64)) == call(view(65536, 16, 1, 128)) == call(view(2, 16, 1 << 30, 128)) == SHAPE
+    assert call(view(65535, 1024, 1, 128), cache(kv_heads=64), width=256) == SHAPE  # the merge's threads
     assert call(view(2, 12, 1, 128)) == call(view(2, 0, 1, 128)) == HEADS
     assert call(width=0) == call(width=(1 << 24) + 1) == call(longest=-1) == PAGES
     assert call(scale=0.0) == call(scale=float("inf")) == call(scale=float("nan")) == SCALE

@@ -396,3 +396,75 @@ def test_attention_strides_streams_and_graphs(ops, tokens):
         eager = ops.paged_attention_kv4(q, cache, t, rows, 0, 0.1)
         torch.cuda.synchronize()
         assert torch.equal(captured, eager)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", SHAPES[:2])
+@pytest.mark.parametrize("rows,tokens", [(65, 1), (130, 1), (70, 3), (67, 40), (64, 40)])
+def test_attention_of_many_rows(ops, heads, kv_heads, dim, rows, tokens):
+    """Batches past a wave's 64 lanes, which the plan takes 64 rows at a time; a few of the last rows are long."""
+    log(f"paged_attention_kv4 rows={rows} {heads}/{kv_heads}/{dim} T={tokens}")
+    g = torch.Generator().manual_seed(rows + tokens)
+    counts = torch.randint(0, tokens + 1, (rows,), generator=g)
+    lengths = counts + torch.randint(0, 100, (rows,), generator=g)
+    lengths[-3:] = torch.tensor([1500, 70, 2500])
+    counts[-3:] = torch.tensor([tokens, 0, tokens])
+    table, pages = make_table(g, lengths.tolist(), 64)
+    cache = filled_cache(ops, g, pages, kv_heads, 64, dim)
+    q = randn(g, rows, heads, tokens, dim)
+    state = torch.stack((counts, lengths)).to(torch.int32)
+    out = ops.paged_attention_kv4(q.cuda(), cache, table.cuda(), state.cuda(), 2500, dim**-0.5)
+    check_attention(out, q, cache, table, state, dim**-0.5)
+
+
+@pytest.mark.parametrize("tokens", [4, 30])
+def test_a_bound_below_the_new_tokens(ops, tokens):
+    """``max_length`` below a row's count: only that many queries are answered, the others are zeros."""
+    log(f"paged_attention_kv4 bound below T={tokens}")
+    g = torch.Generator().manual_seed(8)
+    table, pages = make_table(g, [100, 100], 64)
+    cache = filled_cache(ops, g, pages, 2, 64, 128)
+    q = randn(g, 2, 4, tokens, 128)
+    state = torch.tensor([[tokens, 1], [100, 100]], dtype=torch.int32)
+    out = ops.paged_attention_kv4(q.cuda(), cache, table.cuda(), state.cuda(), 3, 0.1)
+    check_attention(out, q, cache, table, state, 0.1, max_length=3)
+    assert not out[0, 3:].any()
+
+
+@pytest.mark.parametrize("tokens", [1, 24])
+def test_attention_copies_odd_strides(ops, tokens):
+    log(f"paged_attention_kv4 odd strides T={tokens}")
+    g = torch.Generator().manual_seed(11)
+    table, pages = make_table(g, [90, 40], 64)
+    cache = filled_cache(ops, g, pages, 8, 64, 128)
+    q = randn(g, 2, 16, tokens, 128).cuda()
+    wide = torch.full((2, 16, tokens, 131), float("nan"), dtype=torch.bfloat16, device="cuda")
+    wide[..., 1:129] = q
+    state = torch.tensor([[tokens, tokens], [90, 40]], dtype=torch.int32, device="cuda")
+    want = ops.paged_attention_kv4(q, cache, table.cuda(), state, 0, 0.1)
+    assert torch.equal(ops.paged_attention_kv4(wide[..., 1:129], cache, table.cuda(), state, 0, 0.1), want)
+
+
+def test_a_cache_past_32_bits(ops):
+    """Pages behind the first 4 GiB of codes: what is written, read and attended is what a small cache gives."""
+    log("paged kv4 cache past 32 bits")
+    g = torch.Generator().manual_seed(12)
+    heads, size, dim, pages = 8, 256, 256, (1 << 14) + 300  # 256 KiB of codes a page
+    places = [pages - 1, 5, (1 << 14) + 1]
+    big, small = ops.paged_kv4_cache(pages, heads, size, dim, "cuda"), ops.paged_kv4_cache(3, heads, size, dim, "cuda")
+    at = torch.arange(3 * size).reshape(3, size)
+    far = torch.tensor(places)[:, None] * size + at % size
+    x = [randn(g, 3, size, heads, dim).cuda() for _ in range(3)]
+    weight, turn = torch.ones(dim, dtype=torch.bfloat16, device="cuda"), torch.ones(3, size, 64, dtype=torch.bfloat16, device="cuda")
+    queries = [ops.qk_norm_rope_append_kv4(x[0], x[1], x[2], weight, weight, 1e-6, 0.0, turn, turn, s.cuda(), c)
+               for s, c in ((far, big), (at, small))]
+    assert torch.equal(*queries)
+    for a, b in zip(ops.read_kv4(big, far.cuda()), ops.read_kv4(small, at.cuda())):
+        assert torch.equal(a, b) and a.any()
+    for b, s in zip(big, small):
+        assert torch.equal(b[places], s)
+    for tokens in (1, 100):
+        q = queries[0][:1, :, :tokens]
+        state = torch.tensor([[tokens], [3 * size]], dtype=torch.int32, device="cuda")
+        outs = [ops.paged_attention_kv4(q, c, torch.tensor([t], dtype=torch.int32, device="cuda"), state, 0, 0.1)
+                for c, t in ((big, places), (small, [0, 1, 2]))]
+        assert torch.equal(*outs) and outs[0].any()

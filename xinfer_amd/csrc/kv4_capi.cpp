@@ -13,6 +13,9 @@ namespace {
 
 constexpr int64_t kIntMax = std::numeric_limits<int32_t>::max();
 constexpr int64_t kMostTokens = int64_t(1) << 30;  // of a page table's row: positions stay in 32 bits
+constexpr int64_t kMostRows = 65535;               // of a batch
+// A launch's threads are counted in 32 bits.
+bool launchable(int64_t threads) { return threads < (int64_t(1) << 32) - 1024; }
 
 bool aligned16(const void *p) { return p != nullptr && (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
@@ -38,13 +41,13 @@ bool rows_ok(const xinfer_view4 &t) {
   return true;
 }
 
-// key/value [B, Hkv, T, D] of the cache; B * T * heads rows are counted in 32 bits.
+// key/value [B, Hkv, T, D] of the cache; D / 8 threads take each of B * T * heads rows.
 bool new_tokens_ok(const xinfer_view4 &key, const xinfer_view4 &value, const Kv4Cache &cache, int64_t heads) {
   for (int i = 0; i < 4; ++i)
     if (key.size[i] < 0 || value.size[i] != key.size[i]) return false;
   return key.size[1] == cache.Hkv && key.size[3] == cache.D && key.size[0] <= kIntMax && key.size[2] <= kIntMax &&
          (key.size[0] == 0 || key.size[2] <= kIntMax / key.size[0]) &&
-         key.size[0] * key.size[2] <= (kIntMax - 1024) / heads;
+         key.size[0] * key.size[2] <= kIntMax / heads && launchable(key.size[0] * key.size[2] * heads * (cache.D / 8));
 }
 
 View view_of(const xinfer_view4 &t) {
@@ -90,12 +93,19 @@ PagedLaunch paged_decode_launch(const PagedArgs &shapes, int vectors_max, int ti
   return paged_launch(shapes, 0, vectors_max, tile, spread ? waves : 8, (int)target, 8);
 }
 
+int paged_launchable(const PagedLaunches &call) {
+  return launchable((call.few.items + call.many.items) * 512) &&
+                 launchable(call.few.a.B * (call.few_merges() + call.many_merges()) * kMergeThreads)
+             ? XINFER_OK
+             : XINFER_ERR_KV4_SHAPE;
+}
+
 int paged_call(const xinfer_view4 &q, const xinfer_kv4_cache &cache, int64_t table_width, int64_t max_length,
                PagedLaunches &call) {
   PagedArgs a{};
   if (!cache_of(cache, a.cache)) return XINFER_ERR_KV4_CACHE;
   const int64_t B = q.size[0], Hq = q.size[1], T = q.size[2];
-  if (B < 0 || B > 65535 || T < 0 || q.size[3] != a.cache.D) return XINFER_ERR_KV4_SHAPE;
+  if (B < 0 || B > kMostRows || T < 0 || q.size[3] != a.cache.D) return XINFER_ERR_KV4_SHAPE;
   if (Hq < 1 || Hq > 65535 || Hq % a.cache.Hkv != 0) return XINFER_ERR_HEADS;
   if (table_width < 1 || table_width > kMostTokens >> a.cache.page_shift || max_length < 0) return XINFER_ERR_PAGES;
   // Query vectors and items are counted in 32 bits.
@@ -111,7 +121,7 @@ int paged_call(const xinfer_view4 &q, const xinfer_kv4_cache &cache, int64_t tab
   call.many = PagedLaunch{a, 0, 0, 0};
   if (vectors <= 32) {
     call.few = paged_decode_launch(a, 32, vectors <= 16 ? 16 : columns, true);
-    return XINFER_OK;
+    return paged_launchable(call);
   }
   // Rows of more vectors than a decode item has go to the prefill kernel; one row alone does whatever its count.
   const bool alone = B == 1;
@@ -121,7 +131,7 @@ int paged_call(const xinfer_view4 &q, const xinfer_kv4_cache &cache, int64_t tab
     // A record of 128 vectors is written and read at some 5 TB/s; a group of an item takes about 2 us.
     if (B <= 64) call.many.a.record_groups = kPagedPrefillTile * 8.0f * (float)a.cache.D / 5e6f / 2.0f;
   }
-  return XINFER_OK;
+  return paged_launchable(call);
 }
 
 int done(hipError_t e) { return e == hipSuccess ? XINFER_OK : XINFER_ERR_LAUNCH; }
@@ -143,6 +153,7 @@ int xinfer_paged_kv_reserve(const int32_t *kv_before, const int32_t *kv_lengths,
     return XINFER_ERR_PAGES;
   if (rows < 0 || tokens < 0 || tokens > kIntMax) return XINFER_ERR_ARGUMENT;
   if (rows > kIntMax / table_width) return XINFER_ERR_PAGES;
+  if (rows > kMostRows) return XINFER_ERR_ARGUMENT;
   if (!counters || !new_counters || counters == new_counters) return XINFER_ERR_ARGUMENT;
   if (rows > 0 && (!kv_before || !kv_lengths || !query_lengths || !block_table || !free_pages || !lengths))
     return XINFER_ERR_ARGUMENT;
@@ -201,7 +212,7 @@ int xinfer_qk_norm_rope_append_kv4(const xinfer_view4 *q, const xinfer_view4 *ke
   if (!cache_of(*cache, a.cache)) return XINFER_ERR_KV4_CACHE;
   const int64_t B = key->size[0], T = key->size[2], Hq = q->size[1], R = cos->size[3];
   if (q->size[0] != B || q->size[2] != T || q->size[3] != a.cache.D || Hq < 1 || Hq > 65535 ||
-      !new_tokens_ok(*key, *value, a.cache, Hq + a.cache.Hkv) || R < 16 || R > a.cache.D || R % 16 != 0)
+      !new_tokens_ok(*key, *value, a.cache, Hq + a.cache.Hkv + 128 / (a.cache.D / 8)) || R < 16 || R > a.cache.D || R % 16 != 0)
     return XINFER_ERR_KV4_SHAPE;
   for (const xinfer_view4 *r : {cos, sin})
     if (r->size[0] != B || r->size[1] != 1 || r->size[2] != T || r->size[3] != R) return XINFER_ERR_KV4_SHAPE;

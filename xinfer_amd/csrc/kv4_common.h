@@ -96,9 +96,18 @@ struct PagedLaunch {
   int tiles;      // of a row and KV head, at most
   size_t bytes;   // of the records; 0: no row can be cut
 };
+constexpr int kMergeThreads = 256, kMergeVectors = 4;  // of a merge block, and of a team for rows of many vectors
 struct PagedLaunches {
   PagedLaunch few, many;
   size_t bytes() const { return few.bytes + many.bytes; }
+  // Merge blocks of a row.
+  int64_t few_merges() const {
+    return few.bytes == 0 ? 0 : (int64_t)few.a.cache.Hkv * few.tiles * (few.a.tile < few.a.T * few.a.G ? few.a.tile : few.a.T * few.a.G);
+  }
+  int64_t many_merges() const {
+    const int vectors = kMergeThreads / (many.a.cache.D / 4) * kMergeVectors;
+    return many.bytes == 0 ? 0 : (int64_t)many.a.cache.Hkv * many.tiles * ((many.a.tile + vectors - 1) / vectors);
+  }
 };
 
 // Query vectors a KV head that one decode item takes at most (256 features leave registers for one group of 16).

@@ -3,8 +3,6 @@
 #include "paged_prefill.h"
 #include "launch.h"
 
-#include <algorithm>
-
 namespace xattn {
 
 // Occupancy: one column group of up to 128 features fits 128 registers (four waves a SIMD), the others twice that.
@@ -49,12 +47,10 @@ struct MergedRuns {
 // vectors and many runs: a block takes one vector, its teams every TEAMS-th run, and joins them in LDS.  Prefill rows
 // have many vectors of few runs: a team takes kMergeVectors of them, one after another.  Either way four records are
 // read at a time.
-constexpr int kMergeVectors = 4;
-
 template <int D>
-__global__ void __launch_bounds__(256) paged_merge_kernel(const PagedArgs few, const PagedArgs many, int few_blocks,
+__global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(const PagedArgs few, const PagedArgs many, int few_blocks,
                                                           int few_per_row, int many_per_row) {
-  constexpr int TEAMS = 256 / (D / 4);
+  constexpr int TEAMS = kMergeThreads / (D / 4);
   __shared__ f32x4 outs[TEAMS][D / 4];
   __shared__ f32x2 sums[TEAMS];
   const bool together = (int)blockIdx.x < few_blocks;
@@ -125,12 +121,9 @@ static hipError_t launch_d(const PagedLaunches &l, hipStream_t stream) {
     launch_decode<D, 1, 4>(l.few, stream);
   }
   if (l.bytes() > 0) {
-    constexpr int VECTORS = 256 / (D / 4) * kMergeVectors;
-    const int heads = few.cache.Hkv, rows = few.B;
-    const int few_per_row = l.few.bytes > 0 ? heads * l.few.tiles * std::min(few.tile, few.T * few.G) : 0;
-    const int many_per_row = l.many.bytes > 0 ? heads * l.many.tiles * ((many.tile + VECTORS - 1) / VECTORS) : 0;
-    hipLaunchKernelGGL((paged_merge_kernel<D>), dim3((unsigned)rows * (few_per_row + many_per_row)), dim3(256), 0, stream, few,
-                       many, rows * few_per_row, few_per_row, many_per_row);
+    const int rows = few.B, few_per_row = (int)l.few_merges(), many_per_row = (int)l.many_merges();
+    hipLaunchKernelGGL((paged_merge_kernel<D>), dim3((unsigned)rows * (few_per_row + many_per_row)), dim3(kMergeThreads), 0,
+                       stream, few, many, rows * few_per_row, few_per_row, many_per_row);
   }
   return hipGetLastError();
 }

@@ -54,8 +54,6 @@ def paged_c_shims():
     return {_call(name): [text] for name, text in PAGED_C_SHIMS.items()}
 
 
-
-
 def _call(name):
     """The operator ``name``, loading the library on first use."""
     found = _calls.get(name)
@@ -121,8 +119,8 @@ def qk_norm_rope_append_kv4(q, key, value, q_weight, k_weight, eps, weight_offse
 
     ``q`` bf16 [B,T,Hq,D], ``key``/``value`` bf16 [B,T,Hkv,D]: the projections viewed per head; per row
     x * rsqrt(mean(x^2) + eps) * (weight + weight_offset) (0 for plain RMSNorm weights, 1 for weights stored minus
-    one), then the rotation of the first R features by ``cos``/``sin`` bf16 [B,T,R].  All in fp32; the query is rounded
-    to bf16 once, the key goes to its 4 bits directly.
+    one), then the rotation of the first R features by ``cos``/``sin`` bf16 [B,T,R].  The query is computed in
+    fp32 and rounded to bf16 once; the key goes to its 4 bits directly, in 64 bits where fp32 could decide a code.
     """
     return _call("qk_norm_rope_append_kv4")(q, key, value, q_weight, k_weight, eps, weight_offset, cos, sin,
                                           slots, *cache)
