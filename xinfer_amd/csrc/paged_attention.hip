@@ -9,25 +9,40 @@ namespace xattn {
 template <int D, int NC, int WAVES>
 __global__ void __launch_bounds__(64 * WAVES, D == 256 || NC == 2 ? 2 : 4) paged_decode_kernel(const PagedArgs a) {
   __shared__ __attribute__((aligned(1024))) char smem[kPagedDecodeLds<D, WAVES>];
-  paged_decode_item<D, NC, WAVES>(a, blockIdx.x, smem);
+  PagedItem it;
+  if (paged_item(a, paged_lane_row(a, 0), blockIdx.x, it)) paged_decode_item<D, NC, WAVES>(a, blockIdx.x, it, smem);
 }
 
-// Blocks below `few_blocks` take a decode item, the others a prefill item.
 template <int D>
-__global__ void __launch_bounds__(64 * kPagedChunkWaves, 2) paged_both_kernel(const PagedArgs few, const PagedArgs many, int few_blocks) {
+__device__ __forceinline__ void paged_prefill_item(const PagedArgs &a, int index, const PagedItem &it, char *smem) {
+  if constexpr (D == 256) paged_chunk_item_wide<D>(a, index, it, smem);
+  else paged_chunk_item<D>(a, index, it, smem);
+}
+
+// Prefill items first, the much shorter decode items behind them, where they fill what the last prefill items leave idle,
+// then the blocks without an item.  (A batch of 5 chunks and 3 single tokens, 256 features: 432 us, with the decode
+// items first 447.)
+template <int D>
+__global__ void __launch_bounds__(64 * kPagedChunkWaves, 2) paged_both_kernel(const PagedArgs few, const PagedArgs many) {
   constexpr int WAVES = kPagedChunkWaves, CHUNK = kPagedChunkLds<D>, DECODE = kPagedDecodeLds<D, WAVES>;
   __shared__ __attribute__((aligned(1024))) char smem[CHUNK > DECODE ? CHUNK : DECODE];
-  if ((int)blockIdx.x < few_blocks) paged_decode_item<D, paged_decode_columns(D) / 16, WAVES>(few, blockIdx.x, smem);
-  else if constexpr (D == 256) paged_chunk_item_wide<D>(many, blockIdx.x - few_blocks, smem);
-  else paged_chunk_item<D>(many, blockIdx.x - few_blocks, smem);
+  PagedItem it;
+  int index = blockIdx.x;
+  const PagedRow lane_row = paged_lane_row(many, 0);
+  if (paged_item(many, lane_row, index, it)) {
+    paged_prefill_item<D>(many, index, it, smem);
+  } else {
+    index -= it.begin;
+    if (paged_item(few, lane_row, index, it)) paged_decode_item<D, paged_decode_columns(D) / 16, WAVES>(few, index, it, smem);
+  }
 }
 
 // Prefill items alone.
 template <int D>
 __global__ void __launch_bounds__(64 * kPagedChunkWaves, 2) paged_prefill_kernel(const PagedArgs a) {
   __shared__ __attribute__((aligned(1024))) char smem[kPagedChunkLds<D>];
-  if constexpr (D == 256) paged_chunk_item_wide<D>(a, blockIdx.x, smem);
-  else paged_chunk_item<D>(a, blockIdx.x, smem);
+  PagedItem it;
+  if (paged_item(a, paged_lane_row(a, 0), blockIdx.x, it)) paged_prefill_item<D>(a, blockIdx.x, it, smem);
 }
 
 // The running maximum, sum and output (four features) of records read so far.
@@ -112,7 +127,7 @@ static hipError_t launch_d(const PagedLaunches &l, hipStream_t stream) {
   const dim3 block(64 * kPagedChunkWaves);
   const PagedArgs &few = l.few.a, &many = l.many.a;
   if (l.few.items > 0 && l.many.items > 0) {
-    hipLaunchKernelGGL((paged_both_kernel<D>), dim3(l.few.items + l.many.items), block, 0, stream, few, many, (int)l.few.items);
+    hipLaunchKernelGGL((paged_both_kernel<D>), dim3(l.few.items + l.many.items), block, 0, stream, few, many);
   } else if (l.many.items > 0) {
     hipLaunchKernelGGL((paged_prefill_kernel<D>), dim3(l.many.items), block, 0, stream, many);
   } else if (few.tile == 32) {

@@ -208,16 +208,14 @@ __device__ __forceinline__ void paged_scores(const GroupLoads<D> &in, const Quer
 template <int D, int WAVES>
 constexpr int kPagedDecodeLds = WAVES * (PagedShape<D>::STAGE + 16 * 8);
 
-// Item `index` of the plan, by the whole block; smem: kPagedDecodeLds bytes, 1024-byte aligned.
+// Item `it` of the plan, its `index`th, by the whole block; smem: kPagedDecodeLds bytes, 1024-byte aligned.
 template <int D, int NC, int WAVES>
-__device__ __forceinline__ void paged_decode_item(const PagedArgs &a, int index, char *smem) {
+__device__ __forceinline__ void paged_decode_item(const PagedArgs &a, int index, const PagedItem &it, char *smem) {
   using S = PagedShape<D>;
   constexpr int COLS = 16 * NC, THREADS = 64 * WAVES;
   f32x2 *const wave_ml = reinterpret_cast<f32x2 *>(smem + WAVES * S::STAGE);
   const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  PagedItem it;
-  if (!paged_item(a, index, it)) return;
   if (it.count < a.T) paged_zero_padded<D, THREADS>(a, it);
   if (it.count == 0) return;
   const int vectors = min(it.count * a.G - it.tile * COLS, COLS);

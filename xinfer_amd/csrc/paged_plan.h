@@ -24,6 +24,12 @@ __device__ __forceinline__ PagedRow paged_row(const PagedArgs &a, int r) {
   return p;
 }
 
+// The lane's row of 64 from `base` on.
+__device__ __forceinline__ PagedRow paged_lane_row(const PagedArgs &a, int base) {
+  const int r = base + (int)(threadIdx.x & 63);
+  return r < a.B ? paged_row(a, r) : PagedRow{0, 0};
+}
+
 struct PagedItem {
   int row, count, length;
   int h, tile, split, nsplit, tiles;
@@ -51,14 +57,10 @@ __device__ __forceinline__ PagedShare paged_share(const PagedArgs &a, const Page
 struct PagedRows {
   PagedRow p;
   PagedShare s;
-  __device__ __forceinline__ void load(const PagedArgs &a, int base) {
-    const int r = base + (int)(threadIdx.x & 63);
-    p = PagedRow{0, 0};
-    s = PagedShare{0, 0};
-    if (r < a.B) {
-      p = paged_row(a, r);
-      s = paged_share(a, p);
-    }
+  __device__ __forceinline__ void load(const PagedArgs &a, int base) { take(a, base, paged_lane_row(a, base)); }
+  __device__ __forceinline__ void take(const PagedArgs &a, int base, const PagedRow &row) {
+    p = row;
+    s = base + (int)(threadIdx.x & 63) < a.B ? paged_share(a, p) : PagedShare{0, 0};
   }
 };
 
@@ -116,11 +118,12 @@ __device__ __forceinline__ void paged_take(PagedItem &it, const PagedRows &rows,
   it.group_end = __builtin_amdgcn_readlane(rows.s.groups, at);
 }
 
-// Item `index` of the plan; false past its last.  Every lane of a wave calls it, with the same index.
-__device__ __forceinline__ bool paged_item(const PagedArgs &a, int index, PagedItem &it) {
+// Item `index` of the plan; false past its last, it.begin is then how many there are.  Every lane of a wave calls it, with
+// the same index and its row of the first 64.
+__device__ __forceinline__ bool paged_item(const PagedArgs &a, const PagedRow &lane_row, int index, PagedItem &it) {
   const int Hkv = a.cache.Hkv;
   PagedRows rows;
-  rows.load(a, 0);
+  rows.take(a, 0, lane_row);
   const int run = paged_run(a, rows);
   for (int base = 0, before = 0;;) {
     const int nsplit = paged_splits(rows.s, run), items = rows.s.tiles * nsplit * Hkv, upto = before + wave_scan(items);
@@ -140,8 +143,11 @@ __device__ __forceinline__ bool paged_item(const PagedArgs &a, int index, PagedI
       return true;
     }
     base += 64;
-    if (base >= a.B) return false;
     before = __builtin_amdgcn_readlane(upto, 63);
+    if (base >= a.B) {
+      it.begin = before;
+      return false;
+    }
     rows.load(a, base);
   }
 }

@@ -53,16 +53,14 @@ __device__ __forceinline__ void staged_barrier() { asm volatile("s_waitcnt lgkmc
 template <int D>
 constexpr int kPagedChunkLds = D == 256 ? 3 * 64 * 2 * D : 4 * 64 * 2 * D + 64 * kChunkWaves * 8;
 
-// Item `index` of the plan, by the whole block; smem: kPagedChunkLds bytes, 1024-byte aligned.
+// Item `it` of the plan, its `index`th, by the whole block; smem: kPagedChunkLds bytes, 1024-byte aligned.
 template <int D>
-__device__ __forceinline__ void paged_chunk_item(const PagedArgs &a, int index, char *smem) {
+__device__ __forceinline__ void paged_chunk_item(const PagedArgs &a, int index, const PagedItem &it, char *smem) {
   using S = ChunkShape<D>;
   constexpr int COLS = 32 * kChunkWaves;
   const int tid = threadIdx.x & (kChunkThreads - 1), lane = tid & 63, m = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int side = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kChunkThreads);  // which groups: every other one
-  PagedItem it;
-  if (!paged_item(a, index, it)) return;
   paged_zero_padded<D, 2 * kChunkThreads>(a, it);
 
   // This wave's queries.
@@ -325,14 +323,12 @@ __device__ __forceinline__ void paged_chunk_item(const PagedArgs &a, int index, 
 
 // The same for 256 features: 8 waves of 16 query vectors.
 template <int D>
-__device__ __forceinline__ void paged_chunk_item_wide(const PagedArgs &a, int index, char *smem) {
+__device__ __forceinline__ void paged_chunk_item_wide(const PagedArgs &a, int index, const PagedItem &it, char *smem) {
   using S = PagedShape<D>;
   constexpr int WAVES = kPagedChunkWaves, THREADS = 64 * WAVES, COLS = 16 * WAVES, BLOCKS = D / 32, STAGE = 64 * S::ROW;
   static_assert(64 * BLOCKS == THREADS, "a thread stages one block of one key");
   const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  PagedItem it;
-  if (!paged_item(a, index, it)) return;
   paged_zero_padded<D, THREADS>(a, it);
 
   const int vectors = it.count * a.G, wave_first = it.tile * COLS + 16 * wave, j = wave_first + m;
