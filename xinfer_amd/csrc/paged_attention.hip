@@ -57,12 +57,40 @@ struct MergedRuns {
   }
 };
 
+// Runs begin, begin + stride, ... of N vectors, the first at record `at`, the others TEAMS apart (or at `spare`, if nearer).
+// The records of four runs are read together.
+template <int D, int N>
+__device__ __forceinline__ void merge_runs(const PagedArgs &a, int64_t at, int spare, int64_t step, int begin, int stride,
+                                           int nsplit, int f, MergedRuns (&r)[N]) {
+  constexpr int TEAMS = kMergeThreads / (D / 4);
+#pragma unroll
+  for (int n = 0; n < N; ++n) r[n] = MergedRuns{kLowest, 0.0f, f32x4{0.0f, 0.0f, 0.0f, 0.0f}};
+  for (int s0 = begin; s0 < nsplit; s0 += 4 * stride) {
+    f32x2 ml[N][4];
+    f32x4 part[N][4];
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int64_t record = at + min(n * TEAMS, spare) + min(s0 + e * stride, nsplit - 1) * step;
+        ml[n][e] = *as_global(reinterpret_cast<const f32x2 *>(a.part_ml + 2 * record));
+        part[n][e] = *as_global(reinterpret_cast<const f32x4 *>(a.part_o + record * D + 4 * f));
+      }
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (s0 + e * stride < nsplit) r[n].add(ml[n][e].x, ml[n][e].y, part[n][e]);
+  }
+}
+
 // Joins the runs of rows that were cut, of either launch.  D/4 threads side by side take a query vector, 4 features
 // each; a block has 256 / (D/4) such teams.  Decode rows (blocks below few_blocks, the row counting slowest) have few
 // vectors and many runs: a block takes one vector, its teams every TEAMS-th run, and joins them in LDS.  Prefill rows
-// have many vectors of few runs: a team takes kMergeVectors of them, one after another.  Either way four records are
-// read at a time.
-template <int D>
+// have many vectors of few runs: a team takes kMergeVectors of them, N at a time.  N = 4 waits for memory once but leaves
+// three blocks a CU, which pays in a launch of prefill rows alone (512 vectors a head of one row, 4 runs: 6.3 us, with
+// N = 1 7.6) and costs in the others, whose blocks without work are many (64 single tokens: 6.2 us, with N = 1 4.8).
+template <int D, int N>
 __global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(const PagedArgs few, const PagedArgs many, int few_blocks,
                                                           int few_per_row, int many_per_row) {
   constexpr int TEAMS = kMergeThreads / (D / 4);
@@ -83,37 +111,34 @@ __global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(const PagedA
   if (together && (int)first >= vectors) return;
   const int64_t step = (int64_t)a.cache.Hkv * a.tile;
   const int64_t record0 = ((int64_t)it.begin + (int64_t)tile * it.nsplit * a.cache.Hkv + h) * a.tile;
-  const int begin = together ? team : 0, stride = together ? TEAMS : 1;
-  for (int n = 0; n < (together ? 1 : kMergeVectors); ++n) {
-    const int column = together ? first : (first * kMergeVectors + n) * TEAMS + team;
-    if (column >= vectors) return;
-    MergedRuns r{kLowest, 0.0f, f32x4{0.0f, 0.0f, 0.0f, 0.0f}};
-    for (int s0 = begin; s0 < it.nsplit; s0 += 4 * stride) {
-      f32x2 ml[4];
-      f32x4 part[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int64_t record = record0 + column + min(s0 + e * stride, it.nsplit - 1) * step;
-        ml[e] = *as_global(reinterpret_cast<const f32x2 *>(a.part_ml + 2 * record));
-        part[e] = *as_global(reinterpret_cast<const f32x4 *>(a.part_o + record * D + 4 * f));
-      }
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (s0 + e * stride < it.nsplit) r.add(ml[e].x, ml[e].y, part[e]);
-    }
-    if (together) {
-      outs[team][f] = r.out;
-      if (f == 0) sums[team] = f32x2{r.best, r.total};
-      __syncthreads();
-      if (team != 0) return;
-#pragma unroll
-      for (int e = 1; e < TEAMS; ++e) r.add(sums[e].x, sums[e].y, outs[e][f]);
-    }
+  auto finish = [&](const MergedRuns &r, int column) {
     const int j = tile * a.tile + column, t = j / a.G;
-    r.out *= r.total == 0.0f ? 0.0f : 1.0f / r.total;
+    const f32x4 out = r.out * (r.total == 0.0f ? 0.0f : 1.0f / r.total);
     *as_global(reinterpret_cast<u32x2 *>(
         a.out + (((int64_t)row * a.T + t) * a.Hq + h * a.G + (j - t * a.G)) * D + 4 * f)) =
-        u32x2{pack_bf16x2(r.out[0], r.out[1]), pack_bf16x2(r.out[2], r.out[3])};
+        u32x2{pack_bf16x2(out[0], out[1]), pack_bf16x2(out[2], out[3])};
+  };
+  if (together) {
+    MergedRuns r[1];
+    merge_runs<D, 1>(a, record0 + first, 0, step, team, TEAMS, it.nsplit, f, r);
+    outs[team][f] = r[0].out;
+    if (f == 0) sums[team] = f32x2{r[0].best, r[0].total};
+    __syncthreads();
+    if (team != 0) return;
+#pragma unroll
+    for (int e = 1; e < TEAMS; ++e) r[0].add(sums[e].x, sums[e].y, outs[e][f]);
+    finish(r[0], first);
+  } else {
+    for (int n0 = 0; n0 < kMergeVectors; n0 += N) {
+      // Vectors past the row's last are read as the last of the team.
+      const int column = (first * kMergeVectors + n0) * TEAMS + team, spare = vectors - 1 - column;
+      if (spare < 0) return;
+      MergedRuns r[N];
+      merge_runs<D, N>(a, record0 + column, spare, step, 0, 1, it.nsplit, f, r);
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+        if (n * TEAMS <= spare) finish(r[n], column + n * TEAMS);
+    }
   }
 }
 
@@ -137,8 +162,9 @@ static hipError_t launch_d(const PagedLaunches &l, hipStream_t stream) {
   }
   if (l.bytes() > 0) {
     const int rows = few.B, few_per_row = (int)l.few_merges(), many_per_row = (int)l.many_merges();
-    hipLaunchKernelGGL((paged_merge_kernel<D>), dim3((unsigned)rows * (few_per_row + many_per_row)), dim3(kMergeThreads), 0,
-                       stream, few, many, rows * few_per_row, few_per_row, many_per_row);
+    auto merge = l.few.items == 0 ? paged_merge_kernel<D, kMergeVectors> : paged_merge_kernel<D, 1>;
+    hipLaunchKernelGGL(merge, dim3((unsigned)rows * (few_per_row + many_per_row)), dim3(kMergeThreads), 0, stream, few, many,
+                       rows * few_per_row, few_per_row, many_per_row);
   }
   return hipGetLastError();
 }

@@ -46,14 +46,12 @@ __device__ __forceinline__ uint32_t largest(const u32x4 &x, uint32_t top) {
   for (int e = 0; e < 4; ++e) top = max(top, max((x[e] << 16) & 0x7fffffffu, x[e] & 0x7fff0000u));
   return top;
 }
-// Sixteen features (two chunks of bf16) as the two terms, for a block of scale byte `scale`.
-__device__ __forceinline__ void split_query(const u32x4 &x0, const u32x4 &x1, int scale, u32x4 &first, u32x4 &second) {
+// Eight features (bf16) as the two terms, for a block of scale byte `scale`.
+__device__ __forceinline__ void split_query(const u32x4 &x, int scale, u32x2 &first, u32x2 &second) {
   const float unit = kv4_scale_value(min(scale, 254)), small = unit * 0.0625f;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    const u32x4 &x = w < 2 ? x0 : x1;
-    const uint32_t lo = x[2 * (w & 1)], hi = x[2 * (w & 1) + 1];
-    const float f[4] = {bf16_lo(lo), bf16_hi(lo), bf16_lo(hi), bf16_hi(hi)};
+  for (int w = 0; w < 2; ++w) {
+    const float f[4] = {bf16_lo(x[2 * w]), bf16_hi(x[2 * w]), bf16_lo(x[2 * w + 1]), bf16_hi(x[2 * w + 1])};
     i16x2 p{0, 0}, r{0, 0};
     p = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(p, f[0], f[1], unit, false);
     p = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(p, f[2], f[3], unit, true);
@@ -65,6 +63,14 @@ __device__ __forceinline__ void split_query(const u32x4 &x0, const u32x4 &x1, in
     first[w] = word;
     second[w] = __builtin_bit_cast(uint32_t, r);
   }
+}
+// Sixteen (two chunks).
+__device__ __forceinline__ void split_query(const u32x4 &x0, const u32x4 &x1, int scale, u32x4 &first, u32x4 &second) {
+  u32x2 f[2], r[2];
+  split_query(x0, scale, f[0], r[0]);
+  split_query(x1, scale, f[1], r[1]);
+  first = u32x4{f[0].x, f[0].y, f[1].x, f[1].y};
+  second = u32x4{r[0].x, r[0].y, r[1].x, r[1].y};
 }
 
 }  // namespace xattn

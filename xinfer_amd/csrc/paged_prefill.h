@@ -48,10 +48,10 @@ struct Flag {
 // for them, and with that for a memory round trip every group).
 __device__ __forceinline__ void staged_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory"); }
 
-// LDS of a prefill block: staged groups, two for each half of the waves, and the second half's maxima and sums (256
-// features: three groups for all waves).
+// LDS of a prefill block: staged groups, two for each half of the waves, and the queries' terms and scales, later the
+// second half's maxima and sums (256 features: three groups for all waves).
 template <int D>
-constexpr int kPagedChunkLds = D == 256 ? 3 * 64 * 2 * D : 4 * 64 * 2 * D + 64 * kChunkWaves * 8;
+constexpr int kPagedChunkLds = D == 256 ? 3 * 64 * 2 * D : 4 * 64 * 2 * D + kPagedPrefillTile * (2 * D + D / 32);
 
 // Item `it` of the plan, its `index`th, by the whole block; smem: kPagedChunkLds bytes, 1024-byte aligned.
 template <int D>
@@ -75,29 +75,43 @@ __device__ __forceinline__ void paged_chunk_item(const PagedArgs &a, int index, 
   const int tile_end = it.length - it.count + (min(it.tile * COLS + COLS, vectors) - 1) / a.G + 1;
   const int group_end = min(it.group_end, (tile_end + kGroupKeys - 1) / kGroupKeys);
 
-  u32x4 first[S::KS][2], second[S::KS][2], qx[S::KS][2][2];
+  // The block's queries are read row by row, 8 features a lane, turned into their terms once for both halves and
+  // passed through LDS; each wave reading its own would touch a line for every 16 or 32 bytes, and twice.
+  // 16-byte chunk c of vector v's terms lies at c ^ v.
+  constexpr int LANES = D / 8, LOADS = COLS * LANES / (2 * kChunkThreads), SPREAD = D / 16 - 1;
+  char *const terms = smem + 4 * S::STAGE;
+  uint8_t *const scales = reinterpret_cast<uint8_t *>(terms + 2 * COLS * D);
+  const int load_first = threadIdx.x / LANES, load_chunk = threadIdx.x % LANES;
+  u32x4 first[S::KS][2], second[S::KS][2], qx[LOADS];
   int qscale[S::KS];
-  {
-    const uint16_t *const q = a.q.p + it.row * a.q.sb + head * a.q.sh + t * a.q.st;
 #pragma unroll
-    for (int s = 0; s < S::KS; ++s)
-#pragma unroll
-      for (int p = 0; p < 2; ++p)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) qx[s][p][e] = there ? load16(q + 64 * s + 32 * p + 16 * h + 8 * e) : u32x4{0, 0, 0, 0};
+  for (int n = 0; n < LOADS; ++n) {
+    const int i = it.tile * COLS + load_first + n * (COLS / LOADS), token = i / a.G;
+    const uint16_t *const q = a.q.p + it.row * a.q.sb + (it.h * a.G + (i - token * a.G)) * a.q.sh + token * a.q.st;
+    qx[n] = i < vectors ? load16(q + 8 * load_chunk) : u32x4{0, 0, 0, 0};
   }
   auto convert_queries = [&]() {
 #pragma unroll
+    for (int n = 0; n < LOADS; ++n) {
+      const int i = load_first + n * (COLS / LOADS), scale = query_scale(quad_max(largest(qx[n], 0u)));
+      u32x2 x, rest;
+      split_query(qx[n], scale, x, rest);
+      char *const to = terms + i * D + ((load_chunk >> 1) ^ (i & SPREAD)) * 16 + 8 * (load_chunk & 1);
+      *reinterpret_cast<u32x2 *>(to) = x;
+      *reinterpret_cast<u32x2 *>(to + COLS * D) = rest;
+      if (load_chunk % 4 == 0) scales[i * (D / 32) + load_chunk / 4] = (uint8_t)scale;
+    }
+    staged_barrier();
+    const int i = 32 * wave + m;
+#pragma unroll
     for (int s = 0; s < S::KS; ++s) {
-      int b[2];
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
-        const uint32_t top = largest(qx[s][p][1], largest(qx[s][p][0], 0u));
-        const auto r = __builtin_amdgcn_permlane32_swap(top, top, false, false);  // the block's other half
-        b[p] = query_scale(max(r[0], r[1]));
-        split_query(qx[s][p][0], qx[s][p][1], b[p], first[s][p], second[s][p]);
+        const char *const from = terms + i * D + ((4 * s + 2 * p + h) ^ (i & SPREAD)) * 16;
+        first[s][p] = *reinterpret_cast<const u32x4 *>(from);
+        second[s][p] = *reinterpret_cast<const u32x4 *>(from + COLS * D);
       }
-      const int mine = h == 0 ? b[0] : b[1];
+      const int mine = scales[i * (D / 32) + 2 * s + h];
       qscale[s] = mine | (mine == 255 ? 255 : mine - 4) << 8;
     }
   };
