@@ -416,6 +416,23 @@ def test_attention_of_many_rows(ops, heads, kv_heads, dim, rows, tokens):
     check_attention(out, q, cache, table, state, dim**-0.5)
 
 
+@pytest.mark.parametrize("heads,kv_heads,dim,longest", [(16, 8, 128, 600), (16, 8, 128, 768), (16, 8, 64, 1024), (8, 8, 64, 1300),
+                                                        (16, 8, 128, 1025)])
+@pytest.mark.parametrize("rows", [1, 20])
+def test_attention_of_short_rows(ops, heads, kv_heads, dim, longest, rows):
+    """Single tokens over rows that a block takes whole, with its waves' shares from none to two groups."""
+    log(f"paged_attention_kv4 short rows={rows} {heads}/{kv_heads}/{dim} L={longest}")
+    g = torch.Generator().manual_seed(longest)
+    lengths = torch.randint(0, longest + 1, (rows,), generator=g)
+    lengths[-1] = longest
+    table, pages = make_table(g, lengths.tolist(), 64)
+    cache = filled_cache(ops, g, pages, kv_heads, 64, dim)
+    q = randn(g, rows, heads, 1, dim)
+    state = torch.stack((lengths.clamp(max=1), lengths)).to(torch.int32)
+    out = ops.paged_attention_kv4(q.cuda(), cache, table.cuda(), state.cuda(), longest, dim**-0.5)
+    check_attention(out, q, cache, table, state, dim**-0.5)
+
+
 @pytest.mark.parametrize("tokens", [4, 30])
 def test_a_bound_below_the_new_tokens(ops, tokens):
     """``max_length`` below a row's count: only that many queries are answered, the others are zeros."""

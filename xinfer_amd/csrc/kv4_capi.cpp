@@ -56,6 +56,7 @@ View view_of(const xinfer_view4 &t) {
 
 // Launches and workspace of a paged attention call come from the shapes and the bound on the lengths alone.
 constexpr int kPagedCus = 256;
+constexpr int kRowGroups = 1;  // 64-key groups a wave of a decode block that takes a whole row
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
@@ -63,7 +64,7 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // cut, as the merge's launch costs more than it saves.
 PagedLaunch paged_launch(const PagedArgs &shapes, int vectors_min, int vectors_max, int tile, int min_groups, int target,
                          int whole_groups) {
-  PagedLaunch l{shapes, 0, 0, 0};
+  PagedLaunch l{shapes, 0, 0, 0, 8};
   l.a.vectors_min = vectors_min;
   l.a.vectors_max = vectors_max;
   l.a.tile = tile;
@@ -84,17 +85,28 @@ PagedLaunch paged_launch(const PagedArgs &shapes, int vectors_min, int vectors_m
 // of 1024 keys: runs of one group 10.8 us, of two 12.1.)  Two column groups: blocks of 8 waves, one a CU, all at once
 // (six tokens in 8 rows, 32 / 8 heads: 25.4 us, with 4 waves and two blocks a CU 27.5).  In a prefill launch: its
 // blocks' 8 waves.
+//
+// Rows of 9 to some 16 groups, in no more blocks than CUs, are not cut: a block of all 16 waves a CU holds spares the merge's
+// launch, but the CU needs 0.35 us a group (64 features: 0.2), so the limit is higher where the cut rows' groups would
+// share CUs too.  (128 features, 8 KV heads, 12 groups: 1 row 10.4 us, cut 10.3; 16 rows 11.0, cut 11.9; 32 rows 11.8, cut
+// 14.6.  16 groups: 16 rows 12.4, cut 12.1; 24 rows 12.8, cut 14.8.  64 features, 16 groups: 1 row 8.4, cut 9.1; 32 rows
+// 9.3, cut 12.1.  256 features hold 8 waves only, 16 groups: 15.7, cut 12.3.)
 PagedLaunch paged_decode_launch(const PagedArgs &shapes, int vectors_max, int tile, bool alone) {
   const int64_t whole = (int64_t)shapes.B * shapes.cache.Hkv * ceil_div(std::min(shapes.T * shapes.G, vectors_max), tile);
-  const int waves = alone && tile == 16 ? 4 : 8;
+  const int64_t groups = ceil_div(shapes.max_length, 64);
+  const int row_groups = (shapes.cache.D == 64 ? 16 : 12) * (whole > kPagedCus / 2 ? 4 : 3) / 3;
+  const bool rows = alone && tile == 16 && shapes.cache.D < 256 && whole <= kPagedCus && groups > 8 && groups <= row_groups;
+  const int waves = rows ? kPagedRowWaves : alone && tile == 16 ? 4 : 8;
   const int64_t resident = kPagedCus * (waves == 8 ? 1 : shapes.cache.D == 256 ? 2 : 4);
   const int64_t target = waves == 4 ? resident : std::max(resident - whole, resident / 2);
   const bool spread = waves == 4 && whole * ceil_div(shapes.max_length, 64 * waves) <= kPagedCus;
-  return paged_launch(shapes, 0, vectors_max, tile, spread ? waves : 8, (int)target, 8);
+  PagedLaunch l = paged_launch(shapes, 0, vectors_max, tile, spread ? waves : 8, (int)target, rows ? (int)groups : 8);
+  l.waves = waves;
+  return l;
 }
 
 int paged_launchable(const PagedLaunches &call) {
-  return launchable((call.few.items + call.many.items) * 512) &&
+  return launchable((call.few.items + call.many.items) * 1024) &&
                  launchable(call.few.a.B * (call.few_merges() + call.many_merges()) * kMergeThreads)
              ? XINFER_OK
              : XINFER_ERR_KV4_SHAPE;
@@ -118,14 +130,14 @@ int paged_call(const xinfer_view4 &q, const xinfer_kv4_cache &cache, int64_t tab
   a.width = (int32_t)table_width;
   a.max_length = (int32_t)(max_length == 0 ? capacity : std::min(max_length, capacity));
   const int columns = paged_decode_columns(a.cache.D), vectors = a.T * a.G;
-  call.many = PagedLaunch{a, 0, 0, 0};
+  call.many = PagedLaunch{a, 0, 0, 0, 8};
   if (vectors <= 32) {
     call.few = paged_decode_launch(a, 32, vectors <= 16 ? 16 : columns, true);
     return paged_launchable(call);
   }
   // Rows of more vectors than a decode item has go to the prefill kernel; one row alone does whatever its count.
   const bool alone = B == 1;
-  call.few = alone ? PagedLaunch{a, 0, 0, 0} : paged_decode_launch(a, columns, columns, false);
+  call.few = alone ? PagedLaunch{a, 0, 0, 0, 8} : paged_decode_launch(a, columns, columns, false);
   call.many = paged_launch(a, alone ? 0 : columns + 1, kIntMax, kPagedPrefillTile, 8, alone || B > 64 ? kPagedCus : 3 * kPagedCus, 8);
   if (!alone) {
     // A record of 128 vectors is written and read at some 5 TB/s; a group of an item takes about 2 us.

@@ -95,6 +95,7 @@ struct PagedLaunch {
   int64_t items;  // of the plan, at most: blocks, and records; 0: no launch
   int tiles;      // of a row and KV head, at most
   size_t bytes;   // of the records; 0: no row can be cut
+  int waves;      // of a decode block
 };
 constexpr int kMergeThreads = 256, kMergeVectors = 4;  // of a merge block, and of a team for rows of many vectors
 struct PagedLaunches {
@@ -112,6 +113,7 @@ struct PagedLaunches {
 
 // Query vectors a KV head that one decode item takes at most (256 features leave registers for one group of 16).
 constexpr int paged_decode_columns(int dim) { return dim == 256 ? 16 : 32; }
+constexpr int kPagedRowWaves = 16;      // of a decode block that takes a whole row: all that a CU holds (up to 128 features)
 constexpr int kPagedPrefillTile = 128;  // query vectors of a prefill item
 
 }  // namespace xattn

@@ -157,6 +157,8 @@ static hipError_t launch_d(const PagedLaunches &l, hipStream_t stream) {
     hipLaunchKernelGGL((paged_prefill_kernel<D>), dim3(l.many.items), block, 0, stream, many);
   } else if (few.tile == 32) {
     if constexpr (paged_decode_columns(D) == 32) launch_decode<D, 2, 8>(l.few, stream);
+  } else if (l.few.waves == kPagedRowWaves) {
+    if constexpr (D < 256) launch_decode<D, 1, kPagedRowWaves>(l.few, stream);
   } else {
     launch_decode<D, 1, 4>(l.few, stream);
   }
