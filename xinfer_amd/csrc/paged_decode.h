@@ -13,6 +13,11 @@
 //
 // Weights are rounded to bf16.  With up to 8 vectors the other 8 columns hold what that rounding loses
 // (w - bf16(w)), at no further matrix work, which leaves 2^-17 of a weight; with more the rounding is up to 2^-9.
+//
+// What bounds it: memory where there is much to read (64 rows of 1605 to 16384 keys, 16 / 8 heads of 128 features: 637 MB
+// in 141 us, 4.5 TB/s; 8 rows of 55 to 13312 keys, 34 MB: 17.7 us, 4 of them the merge), the vector unit close behind (a
+// wave's group takes some 200 vector instructions, 64 conversions and 16 exponentials, 0.35 us of a CU each in the end),
+// and latency where there is little (one row of 1 to 64 keys 6.1 us, 1024 keys 10.6 with the merge).
 #pragma once
 
 #include "paged_mfma.h"
@@ -221,6 +226,8 @@ __device__ __forceinline__ void paged_decode_item(const PagedArgs &a, int index,
   const int vectors = min(it.count * a.G - it.tile * COLS, COLS);
   const bool twice = NC == 1 && vectors <= 8;  // columns 8..15 repeat the queries and take the weights' rests
 
+  const uint32_t rests = twice && m >= 8 ? ~0u : 0u;
+
   QueryOperand<D> q[NC];
   u32x4 qx[NC][S::KC][QueryOperand<D>::PIECES][2];
   int last_key[NC];  // the last key that this lane's query sees
@@ -307,8 +314,12 @@ __device__ __forceinline__ void paged_decode_item(const PagedArgs &a, int index,
           const int i = 2 * u + w / 2, t = 2 * (w & 1);
           const float p0 = fast_exp2(fmaf(s[n][t][i], a.scale_log2, -now)), p1 = fast_exp2(fmaf(s[n][t + 1][i], a.scale_log2, -now));
           sum[n] += p0 + p1;
-          const uint32_t word = pack_bf16x2(p0, p1);
-          pw[n][u][w] = twice && m >= 8 ? pack_bf16x2(p0 - bf16_lo(word), p1 - bf16_hi(word)) : word;
+          if constexpr (NC == 1) {
+            const uint32_t word = pack_weights(p0, p1) & rests;
+            pw[n][u][w] = pack_weights(p0 - bf16_lo(word), p1 - bf16_hi(word));
+          } else {
+            pw[n][u][w] = pack_weights(p0, p1);
+          }
         }
     }
 

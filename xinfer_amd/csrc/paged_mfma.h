@@ -23,6 +23,11 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef short i16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
+// Two weights as bf16 in one instruction (pack_bf16x2 takes four).
+__device__ __forceinline__ uint32_t pack_weights(float lo, float hi) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{lo, hi}, bf16x2));
+}
+
 template <int OPA, int OPB>
 __device__ __forceinline__ f32x4 mfma16_fp4(const u32x4 &a, const u32x4 (&b)[2], f32x4 c, int scale_a, int scale_b) {
   const i32x8 x{(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0};

@@ -1,11 +1,14 @@
 // Work items of attention over the paged cache, laid out on the device from the rows' lengths.
 //
-// A launch is sized by the shapes alone.  Its waves each compute the same plan from the lengths: a row's keys are
-// cut into `nsplit` runs of 64-key groups, its query vectors (query heads of a KV head times tokens) into tiles, and
-// an item is a (tile, run, KV head).  Runs take at least `min_groups` groups, and as many more as leave at most about
-// `target` items (paged_run), so a few long rows fill the chip and many rows are not cut at all.  Items past the plan's last end
-// at once.  The KV head counts fastest: consecutive blocks go to the 8 XCDs in turn, so with 8 KV heads the tiles
-// of one head meet in one XCD's L2.
+// A launch is sized by the shapes alone.  Its waves each compute the same plan from the lengths: a row's keys are cut into
+// `nsplit` runs of 64-key groups, its query vectors (query heads of a KV head times tokens) into tiles, and an item is a
+// (tile, run, KV head).  Runs take at least `min_groups` groups, and as many more as leave at most about `target` items
+// (paged_run), so a few long rows fill the chip and many rows are not cut at all.  Items past the plan's last end at once.
+// The KV head counts fastest: consecutive blocks go to the 8 XCDs in turn, so with 8 KV heads the tiles of one head meet
+// in one XCD's L2.
+//
+// What bounds it: latency.  A block knows its item some 1.3 us after its start (arguments, lengths, a dozen exchanges
+// among lanes); a block without one holds its place on a CU for about 3 us.
 #pragma once
 
 #include "kv4_device.h"
@@ -71,9 +74,9 @@ __device__ __forceinline__ int paged_splits(const PagedShare &s, int run) { retu
 // Prefill items of ragged batches are long and of different lengths, so what a target of items gives is estimated for
 // eight: n items of at most m groups on kPagedSlots blocks at a time take no longer than ceil(n / slots) m, nor than
 // their mean load and m; an item costs kPagedItemGroups more (queries in, output out) and a record what it is written
-// and read for (a.record_groups).  On a batch of 5 rows of 33 to 223 groups, 256 features: 434 us with the target so
-// found (768), 500 with 512, 515 with 256; on uniform batches 256 is best (4 rows of 64 groups, 128 features: 88 us, 117
-// with 768).
+// and read for (a.record_groups).  On a batch of 5 rows of 33 to 223 groups, 256 features: 432 us with targets up to
+// 768, 499 with 512 or 256; uniform batches choose 256 (4 rows of 64 groups, 128 features: 94 us, with 256 alone 92, the rest
+// being blocks without an item).
 constexpr int kPagedSlots = 256;
 constexpr float kPagedItemGroups = 4.0f;
 

@@ -1,11 +1,12 @@
 // Attention over the paged 4-bit cache for rows of many query vectors a KV head: prompt chunks.
 //
-// A block takes an item (paged_plan.h): 128 query vectors of a (row, KV head) over a run of keys in 64-key groups.  Up
-// to 128 features each half of its 8 waves takes all of them, 32 a wave, over every other group (paged_chunk_item).  A wave reads the group's keys as they lie in the cache, as the A operand of the scaled
-// 32x32x64 product against its queries' two e4m3 terms (paged_mfma.h): row m of tile t (of two) is key 2 m + t, so a
-// lane's two keys have their scales in neighbouring bytes.  A lane (column q, half h) then holds 32 scores of its query,
-// and for each 16 keys 8 neighbouring ones, which is the B operand of the bf16 PV product: nothing of the softmax
-// crosses lanes but the maximum and, at the end, the sum of the two halves.
+// A block takes an item (paged_plan.h): 128 query vectors of a (row, KV head) over a run of keys in 64-key groups.  Up to
+// 128 features each half of its 8 waves takes all of them, 32 a wave, over every other group (paged_chunk_item).  A wave
+// reads the group's keys as they lie in the cache, as the A operand of the scaled 32x32x64 product against its queries'
+// two e4m3 terms (paged_mfma.h): row m of tile t (of two) is key 2 m + t, so a lane's two keys have their scales in
+// neighbouring bytes.  A lane (column q, half h) then holds 32 scores of its query, and for each 16 keys 8 neighbouring
+// ones, which is the B operand of the bf16 PV product: nothing of the softmax crosses lanes but the maximum and, at the
+// end, the sum of the two halves.
 //
 // The waves of a group turn its values into bf16 (exact) in LDS together, a group ahead, and each reads them transposed
 // as the A operand.  One barrier a round.
@@ -15,6 +16,13 @@
 // decode kernel (paged_decode.h) but values staged by the whole block.
 //
 // Weights are rounded to bf16 (2^-9 of a weight at most, on average lost in the sum); their sum is taken before.
+//
+// What bounds it: a round (two groups of 128 vectors, 128 features) takes some 5000 clocks, of which a SIMD's matrix unit
+// works 2050, its vector unit about 2000 (a quarter of that exponentials) and the CU's LDS 1500; two waves a SIMD hide
+// part of one behind the other.  512 tokens in each of 8 rows of 8192 keys, page size 64: 32 / 8 heads of 128 features
+// 0.55 ms (970 TFLOP/s), 16 / 8 heads 0.30 ms (890), 16 / 4 heads of 256 features 0.60 ms (890).  One row of 512 tokens
+// and 2048 keys, 16 / 8 heads: 30.5 us with the merge, of which the rounds are 10, the way to the first (plan, queries,
+// first keys) 5, the records 3 to write and 6 to merge; 64 tiles fill a quarter of the CUs, so it has to be cut.
 #pragma once
 
 #include "paged_decode.h"
@@ -222,7 +230,7 @@ __device__ __forceinline__ void paged_chunk_item(const PagedArgs &a, int index, 
       for (int w = 0; w < 4; ++w) {
         const float p0 = fast_exp2(fmaf(s[0][4 * b + w], a.scale_log2, -top)), p1 = fast_exp2(fmaf(s[1][4 * b + w], a.scale_log2, -top));
         sum += p0 + p1;
-        pw[b][w] = pack_bf16x2(p0, p1);
+        pw[b][w] = pack_weights(p0, p1);
       }
   };
   auto output = [&](int buffer) {
@@ -432,7 +440,7 @@ __device__ __forceinline__ void paged_chunk_item_wide(const PagedArgs &a, int in
         const int i = 2 * u + w / 2, z = 2 * (w & 1);
         const float p0 = fast_exp2(fmaf(s[z][i], a.scale_log2, -top)), p1 = fast_exp2(fmaf(s[z + 1][i], a.scale_log2, -top));
         sum += p0 + p1;
-        pw[u][w] = pack_bf16x2(p0, p1);
+        pw[u][w] = pack_weights(p0, p1);
       }
   };
   auto output = [&](int buffer) {

@@ -9,7 +9,8 @@
 // it again with the same inputs gives the same results; the ring's head and tail are returned, not updated.
 //
 // A block takes one row and scans the demands of all (three numbers each) by itself, so no block waits for another.
-// What bounds it: latency, three dependent reads (lengths; the ring or the table; nothing waits for the stores).
+// What bounds it: latency, three dependent reads (lengths; the ring or the table; nothing waits for the stores) and two
+// barriers: 64 rows of one token 3.7 us, 256 rows of up to 512 tokens (2.1 MB of positions and slots) 4.9 us.
 #include "kv4_device.h"
 #include "launch.h"
 
