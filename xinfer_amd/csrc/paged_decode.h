@@ -12,7 +12,7 @@
 // half a group at a time, to be read transposed.
 //
 // Weights are rounded to bf16.  With up to 8 vectors the other 8 columns hold what that rounding loses
-// (w - bf16(w)), at no further matrix work, which leaves 2^-17 of a weight; with more the rounding is up to 2^-9.
+// (w - bf16(w)), at no further matrix work, which leaves 2^-16 of a weight; with more the rounding is up to 2^-8.
 //
 // What bounds it: memory where there is much to read (64 rows of 1605 to 16384 keys, 16 / 8 heads of 128 features: 637 MB
 // in 141 us, 4.5 TB/s; 8 rows of 55 to 13312 keys, 34 MB: 17.7 us, 4 of them the merge), the vector unit close behind (a

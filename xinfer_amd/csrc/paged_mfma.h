@@ -28,6 +28,12 @@ __device__ __forceinline__ uint32_t pack_weights(float lo, float hi) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{lo, hi}, bf16x2));
 }
 
+// Adds two packed weights to a sum.  The instruction is off by up to 1.5 ulp of the result, on average 0.03 downwards
+// (measured: weights and sums of random exponents against float64), so it is for sums of a few words.
+__device__ __forceinline__ float add_weights(uint32_t word, float sum) {
+  return __builtin_amdgcn_fdot2_f32_bf16(as_bf16x2(word), as_bf16x2(0x3f803f80u), sum, false);
+}
+
 template <int OPA, int OPB>
 __device__ __forceinline__ f32x4 mfma16_fp4(const u32x4 &a, const u32x4 (&b)[2], f32x4 c, int scale_a, int scale_b) {
   const i32x8 x{(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0};
