@@ -42,11 +42,12 @@ struct ChunkShape {
   static constexpr int UNITS = 64 * (D / 32);                        // (key, block) units of a group
 };
 
-// XOR of the 16-byte chunk index of staged row r: the four rows that a half's transposing read takes lie in different
-// quarters of the banks, and so do the blocks and rows that eight storing lanes hold.
+// Slot of 16-byte chunk c of staged row r: c ^ S(r), with 128 features c ^ S(r) ^ 2 (c / 8).  LDS serves 128 bytes a clock.
+// What one takes of a transposing read are two neighbouring chunks of four rows, of a store chunks 4 b + const. of two rows'
+// four blocks (64 features: four rows' two blocks); either lies in eight different slots modulo eight.
 template <int D>
 __device__ __forceinline__ int chunk_swizzle(int r) {
-  return D == 64 ? 5 * ((r >> 1) & 1) : 5 * (r & 3);
+  return D == 64 ? 5 * (r & 1) ^ (r & 2) : 5 * (r & 3);
 }
 
 template <bool B>
@@ -166,7 +167,7 @@ __device__ __forceinline__ void paged_chunk_item(const PagedArgs &a, int index, 
   const uint32_t value_at = 16 * tid, value_scale_at = block * size + row;
   const uint32_t stage = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)smem + side * 2 * S::STAGE;
   const bool stages = S::UNITS == kChunkThreads || tid < S::UNITS;
-  const uint32_t put_at = stage + row * S::ROW + ((4 * block) ^ chunk_swizzle<D>(row)) * 16;
+  const uint32_t put_at = stage + row * S::ROW + ((4 * block) ^ chunk_swizzle<D>(row) ^ (block & 2)) * 16;
   auto load_values = [&](int group, int page) {
     const int64_t hd = (int64_t)max(page, 0) * a.cache.Hkv + it.h;
     const uint8_t *const codes = a.cache.value + (hd * size + place(group)) * (D / 2);
@@ -240,7 +241,7 @@ __device__ __forceinline__ void paged_chunk_item(const PagedArgs &a, int index, 
     pipelined<4 * S::DT, 4>(
         [&](int n) {
           const int b = n / S::DT, d = n % S::DT;
-          const uint32_t at = (get ^ (64 * d)) + 16 * b * S::ROW;
+          const uint32_t at = (get ^ (64 * d) ^ (16 * (d & 2))) + 16 * b * S::ROW;
           const u32x2 lo = read_transposed(at), hi = read_transposed(at + 4 * S::ROW);
           return as_bf16x8(u32x4{lo.x, lo.y, hi.x, hi.y});
         },
@@ -382,12 +383,12 @@ __device__ __forceinline__ void paged_chunk_item_wide(const PagedArgs &a, int in
   };
   auto place = [&](int group) { return (group & ((1 << shift) - 1)) * kGroupKeys; };
 
-  // Staged values: 16-byte chunk c of key r lies at slot c ^ S(r) ^ (c / 16), which spreads over the banks the eight
-  // blocks of a key that eight lanes store, and the 16 rows of a transposing read.
+  // Staged values: 16-byte chunk c of key r lies at slot c ^ S(r) ^ (c / 8), which puts the eight blocks of a key that eight
+  // lanes store, and the chunk pairs of four rows that 16 lanes read, in different slots modulo eight.
   auto swizzle = [](int r) { return 2 * ((r & 3) + 4 * ((r >> 4) & 1)); };
   const int key = tid / BLOCKS, block = tid % BLOCKS;
   const uint32_t stage = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)smem;
-  const uint32_t put_at = stage + key * S::ROW + ((4 * block) ^ swizzle(key) ^ (block >> 2)) * 16;
+  const uint32_t put_at = stage + key * S::ROW + ((4 * block) ^ swizzle(key) ^ (block >> 1)) * 16;
   const int x = 16 * g + (m >> 2);
   uint32_t get_at = stage + x * S::ROW + (((m & 3) >> 1) ^ swizzle(x)) * 16 + 8 * (m & 1);
   u32x4 v;
@@ -452,7 +453,7 @@ __device__ __forceinline__ void paged_chunk_item_wide(const PagedArgs &a, int in
     pipelined<2 * S::DT, 4>(
         [&](int k) {
           const int u = k / S::DT, d = k % S::DT;
-          const uint32_t at = (get ^ (32 * d) ^ (d >= 8 ? 16 : 0)) + 8 * u * S::ROW;
+          const uint32_t at = (get ^ (32 * d) ^ (16 * (d >> 2))) + 8 * u * S::ROW;
           const u32x2 lo = read_transposed(at), hi = read_transposed(at + 4 * S::ROW);
           return as_bf16x8(u32x4{lo.x, lo.y, hi.x, hi.y});
         },
