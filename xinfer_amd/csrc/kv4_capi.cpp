@@ -81,7 +81,7 @@ PagedLaunch paged_launch(const PagedArgs &shapes, int vectors_min, int vectors_m
 
 // Decode blocks and items.  One column group: blocks of 4 waves and items enough to fill the chip (16 waves a CU up to
 // 128 features, 8 of 256), since single waves wait for memory and LDS most of the time; runs of two groups a wave, or of
-// one where all those items have a CU of their own.  (8 ragged rows, 128 features: 17.9 us, with 8 waves 19.2; one row
+// one where all those items have a CU of their own.  (8 ragged rows, 128 features: 17.9 us, with 8 waves 19.2, now 17.0; one row
 // of 1024 keys: runs of one group 10.8 us, of two 12.1.)  Two column groups: blocks of 8 waves, one a CU, all at once
 // (six tokens in 8 rows, 32 / 8 heads: 25.4 us, with 4 waves and two blocks a CU 27.5).  In a prefill launch: its
 // blocks' 8 waves.

@@ -21,7 +21,7 @@ __device__ __forceinline__ void paged_prefill_item(const PagedArgs &a, int index
 
 // Prefill items first, the much shorter decode items behind them, where they fill what the last prefill items leave idle,
 // then the blocks without an item.  (A batch of 5 chunks and 3 single tokens, 256 features: 432 us, with the decode
-// items first 447.)
+// items first 447; 395 now.)
 template <int D>
 __global__ void __launch_bounds__(64 * kPagedChunkWaves, 2) paged_both_kernel(const PagedArgs few, const PagedArgs many) {
   constexpr int WAVES = kPagedChunkWaves, CHUNK = kPagedChunkLds<D>, DECODE = kPagedDecodeLds<D, WAVES>;

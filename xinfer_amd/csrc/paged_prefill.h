@@ -19,12 +19,12 @@
 // 256 features after it, a group's by half as many instructions (5 chunks and 3 single tokens: 411 us, 428 with the
 // sum before; with 128 features it makes no difference).
 //
-// What bounds it: a round (two groups of 128 vectors, 128 features) takes some 5000 clocks, of which a SIMD's matrix unit
-// works 2050, its vector unit about 2000 (a quarter of that exponentials) and the CU's LDS 1500; two waves a SIMD hide
-// part of one behind the other.  512 tokens in each of 8 rows of 8192 keys, page size 64: 32 / 8 heads of 128 features
-// 0.55 ms (970 TFLOP/s), 16 / 8 heads 0.30 ms (890), 16 / 4 heads of 256 features 0.60 ms (890).  One row of 512 tokens
-// and 2048 keys, 16 / 8 heads: 30.5 us with the merge, of which the rounds are 10, the way to the first (plan, queries,
-// first keys) 5, the records 3 to write and 6 to merge; 64 tiles fill a quarter of the CUs, so it has to be cut.
+// What bounds it: matrix and vector unit share a SIMD's issue, and two waves hide little more.  512 tokens in each of 8 rows
+// of 8192 keys, page size 64: 16 / 8 heads of 128 features 0.28 to 0.29 ms (930 TFLOP/s; of the clocks the matrix units work
+// 46 %, the vector units 56 %, a quarter of that exponentials), 32 / 8 heads 0.51 to 0.54 (990 to 1040), 16 / 4 heads of 256
+// features 0.56 (950; 40 and 38 %, the rest waits for LDS and the block's barrier).  One row of 512 tokens and 2048
+// keys, 16 / 8 heads: 30 us with the merge, of which the rounds are 10, the way to the first (plan, queries, first keys) 5,
+// the records 3 to write and 6 to merge; 64 tiles fill a quarter of the CUs, so it has to be cut.
 #pragma once
 
 #include "paged_decode.h"
@@ -450,6 +450,7 @@ __device__ __forceinline__ void paged_chunk_item_wide(const PagedArgs &a, int in
   };
   auto output = [&](int buffer) {
     const uint32_t get = get_at + buffer * STAGE;
+    __builtin_amdgcn_s_setprio(1);  // before the other wave's vector work (5 chunks, 3 single tokens: 395 us, without 407)
     pipelined<2 * S::DT, 4>(
         [&](int k) {
           const int u = k / S::DT, d = k % S::DT;
@@ -461,6 +462,7 @@ __device__ __forceinline__ void paged_chunk_item_wide(const PagedArgs &a, int in
           const int u = k / S::DT, d = k % S::DT;
           o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, as_bf16x8(u32x4{pw[u][0], pw[u][1], pw[u][2], pw[u][3]}), o[d], 0, 0, 0);
         });
+    __builtin_amdgcn_s_setprio(0);
   };
   // Waves w and w + 4 share a SIMD.  Between two barriers the first half of the waves computes weights, then the
   // matrix products (this group's output, the next one's scores); the second half the products first (the last
