@@ -84,7 +84,7 @@ struct PagedArgs {
   int32_t vectors_min, vectors_max;
   int32_t tile, min_groups, target;
   float record_groups;  // cost of a record in groups' time; 0: the target as it is (paged_run)
-  float *part_o;  // [item][tile][D] unnormalised outputs of rows cut into runs
+  float *part_o;  // unnormalised outputs of rows cut into runs: decode [item][tile][D], prefill [item][D / 4][tile][4]
   float *part_ml;  // [item][tile][2] running maximum (log2 units) and sum
 };
 
@@ -97,7 +97,7 @@ struct PagedLaunch {
   size_t bytes;   // of the records; 0: no row can be cut
   int waves;      // of a decode block
 };
-constexpr int kMergeThreads = 256, kMergeVectors = 4;  // of a merge block, and of a team for rows of many vectors
+constexpr int kMergeThreads = 256, kMergeQuads = 4;  // of a merge block; quads of features a thread takes of a prefill row
 struct PagedLaunches {
   PagedLaunch few, many;
   size_t bytes() const { return few.bytes + many.bytes; }
@@ -106,7 +106,7 @@ struct PagedLaunches {
     return few.bytes == 0 ? 0 : (int64_t)few.a.cache.Hkv * few.tiles * (few.a.tile < few.a.T * few.a.G ? few.a.tile : few.a.T * few.a.G);
   }
   int64_t many_merges() const {
-    const int vectors = kMergeThreads / (many.a.cache.D / 4) * kMergeVectors;
+    const int vectors = 4 * kMergeThreads * kMergeQuads / many.a.cache.D;
     return many.bytes == 0 ? 0 : (int64_t)many.a.cache.Hkv * many.tiles * ((many.a.tile + vectors - 1) / vectors);
   }
 };

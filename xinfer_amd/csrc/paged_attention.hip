@@ -21,7 +21,7 @@ __device__ __forceinline__ void paged_prefill_item(const PagedArgs &a, int index
 
 // Prefill items first, the much shorter decode items behind them, where they fill what the last prefill items leave idle,
 // then the blocks without an item.  (A batch of 5 chunks and 3 single tokens, 256 features: 432 us, with the decode
-// items first 447; 395 now.)
+// items first 447; 390 now.)
 template <int D>
 __global__ void __launch_bounds__(64 * kPagedChunkWaves, 2) paged_both_kernel(const PagedArgs few, const PagedArgs many) {
   constexpr int WAVES = kPagedChunkWaves, CHUNK = kPagedChunkLds<D>, DECODE = kPagedDecodeLds<D, WAVES>;
@@ -45,99 +45,99 @@ __global__ void __launch_bounds__(64 * kPagedChunkWaves, 2) paged_prefill_kernel
   if (paged_item(a, paged_lane_row(a, 0), blockIdx.x, it)) paged_prefill_item<D>(a, blockIdx.x, it, smem);
 }
 
-// The running maximum, sum and output (four features) of records read so far.
+// The running maximum, sum and output (N times four features) of a vector's runs so far.
+template <int N>
 struct MergedRuns {
   float best, total;
-  f32x4 out;
-  __device__ __forceinline__ void add(float m, float l, const f32x4 &part) {
+  f32x4 out[N];
+  __device__ __forceinline__ MergedRuns() : best(kLowest), total(0.0f) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) out[n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  __device__ __forceinline__ void add(float m, float l, const f32x4 (&part)[N]) {
     const float now = fmaxf(best, m), old = fast_exp2(best - now), keep = fast_exp2(m - now);
     best = now;
     total = total * old + l * keep;
-    out = out * old + part * keep;
+#pragma unroll
+    for (int n = 0; n < N; ++n) out[n] = out[n] * old + part[n] * keep;
+  }
+  // Runs begin, begin + stride, ...: the first run's record at ml and o, the runs ml_step and o_step apart, quad n of a
+  // record at quad * n.  Four runs are read together.
+  __device__ __forceinline__ void read(const float *ml, const float *o, int64_t ml_step, int64_t o_step, int64_t quad,
+                                       int begin, int stride, int nsplit) {
+    for (int s0 = begin; s0 < nsplit; s0 += 4 * stride) {
+      f32x2 x[4];
+      f32x4 part[4][N];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int64_t s = min(s0 + e * stride, nsplit - 1);
+        x[e] = *as_global(reinterpret_cast<const f32x2 *>(ml + s * ml_step));
+#pragma unroll
+        for (int n = 0; n < N; ++n) part[e][n] = *as_global(reinterpret_cast<const f32x4 *>(o + s * o_step + quad * n));
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (s0 + e * stride < nsplit) add(x[e].x, x[e].y, part[e]);
+    }
   }
 };
 
-// Runs begin, begin + stride, ... of N vectors, the first at record `at`, the others TEAMS apart (or at `spare`, if nearer).
-// The records of four runs are read together.
-template <int D, int N>
-__device__ __forceinline__ void merge_runs(const PagedArgs &a, int64_t at, int spare, int64_t step, int begin, int stride,
-                                           int nsplit, int f, MergedRuns (&r)[N]) {
-  constexpr int TEAMS = kMergeThreads / (D / 4);
-#pragma unroll
-  for (int n = 0; n < N; ++n) r[n] = MergedRuns{kLowest, 0.0f, f32x4{0.0f, 0.0f, 0.0f, 0.0f}};
-  for (int s0 = begin; s0 < nsplit; s0 += 4 * stride) {
-    f32x2 ml[N][4];
-    f32x4 part[N][4];
-#pragma unroll
-    for (int n = 0; n < N; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int64_t record = at + min(n * TEAMS, spare) + min(s0 + e * stride, nsplit - 1) * step;
-        ml[n][e] = *as_global(reinterpret_cast<const f32x2 *>(a.part_ml + 2 * record));
-        part[n][e] = *as_global(reinterpret_cast<const f32x4 *>(a.part_o + record * D + 4 * f));
-      }
-#pragma unroll
-    for (int n = 0; n < N; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (s0 + e * stride < nsplit) r[n].add(ml[n][e].x, ml[n][e].y, part[n][e]);
-  }
-}
-
-// Joins the runs of rows that were cut, of either launch.  D/4 threads side by side take a query vector, 4 features
-// each; a block has 256 / (D/4) such teams.  Decode rows (blocks below few_blocks, the row counting slowest) have few
-// vectors and many runs: a block takes one vector, its teams every TEAMS-th run, and joins them in LDS.  Prefill rows
-// have many vectors of few runs: a team takes kMergeVectors of them, N at a time.  N = 4 waits for memory once but leaves
-// three blocks a CU, which pays in a launch of prefill rows alone (512 vectors a head of one row, 4 runs: 6.3 us, with
-// N = 1 7.6) and costs in the others, whose blocks without work are many (64 single tokens: 6.2 us, with N = 1 4.8).
+// Joins the runs of rows that were cut, of either launch.  Decode rows (blocks below few_blocks, the row counting slowest)
+// have few vectors and many runs: a block takes one vector, D/4 threads side by side four features each, its 256 / (D/4)
+// teams every TEAMS-th run, and joins them in LDS.  Prefill rows have many vectors of few runs: threads side by side take
+// vectors side by side, kMergeQuads quads of features each, N at a time, so records are read in runs of 256 bytes and more.
+// N = 2 leaves eight blocks a CU, for launches with many blocks without work (64 single tokens: 4.9 us, with three blocks a
+// CU 6.2; 92 MB of records of 5 chunks 18.8 us); N = 4 waits for memory once, for prefill rows alone (512 tokens of one
+// row, 17 MB of records: 5.6 us, a vector a team 7.6).
 template <int D, int N>
 __global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(const PagedArgs few, const PagedArgs many, int few_blocks,
-                                                          int few_per_row, int many_per_row) {
-  constexpr int TEAMS = kMergeThreads / (D / 4);
+                                                                    int few_per_row, int many_per_row) {
+  constexpr int TEAMS = kMergeThreads / (D / 4), VECTORS = 4 * kMergeThreads * kMergeQuads / D;
   __shared__ f32x4 outs[TEAMS][D / 4];
   __shared__ f32x2 sums[TEAMS];
   const bool together = (int)blockIdx.x < few_blocks;
   const PagedArgs &a = together ? few : many;
   const uint32_t at = together ? blockIdx.x : blockIdx.x - few_blocks, per_row = together ? few_per_row : many_per_row;
   const uint32_t row = at / per_row, in_row = at - row * per_row;
-  const uint32_t per = together ? min(a.tile, a.T * a.G) : (a.tile + TEAMS * kMergeVectors - 1) / (TEAMS * kMergeVectors);
+  const uint32_t per = together ? min(a.tile, a.T * a.G) : (a.tile + VECTORS - 1) / VECTORS;
   const uint32_t unit = in_row / per, first = in_row - unit * per;
   const int tile = unit / a.cache.Hkv, h = unit - tile * a.cache.Hkv;
   PagedItem it;
   paged_row_items(a, row, it);
   if (it.nsplit <= 1 || tile >= it.tiles) return;
-  const int team = threadIdx.x / (D / 4), f = threadIdx.x % (D / 4);
   const int vectors = min(it.count * a.G - tile * a.tile, a.tile);
-  if (together && (int)first >= vectors) return;
-  const int64_t step = (int64_t)a.cache.Hkv * a.tile;
-  const int64_t record0 = ((int64_t)it.begin + (int64_t)tile * it.nsplit * a.cache.Hkv + h) * a.tile;
-  auto finish = [&](const MergedRuns &r, int column) {
+  const int64_t item = (int64_t)it.begin + (int64_t)tile * it.nsplit * a.cache.Hkv + h;
+  const int64_t ml_step = 2 * (int64_t)a.cache.Hkv * a.tile, o_step = (int64_t)a.cache.Hkv * a.tile * D;
+  // Output of four features from 4 f on.
+  auto finish = [&](int column, int f, const f32x4 &sum, float total) {
     const int j = tile * a.tile + column, t = j / a.G;
-    const f32x4 out = r.out * (r.total == 0.0f ? 0.0f : 1.0f / r.total);
+    const f32x4 out = sum * (total == 0.0f ? 0.0f : 1.0f / total);
     *as_global(reinterpret_cast<u32x2 *>(
         a.out + (((int64_t)row * a.T + t) * a.Hq + h * a.G + (j - t * a.G)) * D + 4 * f)) =
         u32x2{pack_bf16x2(out[0], out[1]), pack_bf16x2(out[2], out[3])};
   };
   if (together) {
-    MergedRuns r[1];
-    merge_runs<D, 1>(a, record0 + first, 0, step, team, TEAMS, it.nsplit, f, r);
-    outs[team][f] = r[0].out;
-    if (f == 0) sums[team] = f32x2{r[0].best, r[0].total};
+    if ((int)first >= vectors) return;
+    const int team = threadIdx.x / (D / 4), f = threadIdx.x % (D / 4);
+    const int64_t record = item * a.tile + first;
+    MergedRuns<1> r;
+    r.read(a.part_ml + 2 * record, a.part_o + record * D + 4 * f, ml_step, o_step, 0, team, TEAMS, it.nsplit);
+    outs[team][f] = r.out[0];
+    if (f == 0) sums[team] = f32x2{r.best, r.total};
     __syncthreads();
     if (team != 0) return;
 #pragma unroll
-    for (int e = 1; e < TEAMS; ++e) r[0].add(sums[e].x, sums[e].y, outs[e][f]);
-    finish(r[0], first);
+    for (int e = 1; e < TEAMS; ++e) r.add(sums[e].x, sums[e].y, {outs[e][f]});
+    finish(first, f, r.out[0], r.total);
   } else {
-    for (int n0 = 0; n0 < kMergeVectors; n0 += N) {
-      // Vectors past the row's last are read as the last of the team.
-      const int column = (first * kMergeVectors + n0) * TEAMS + team, spare = vectors - 1 - column;
-      if (spare < 0) return;
-      MergedRuns r[N];
-      merge_runs<D, N>(a, record0 + column, spare, step, 0, 1, it.nsplit, f, r);
+    const int column = first * VECTORS + threadIdx.x % VECTORS, f = kMergeQuads * (threadIdx.x / VECTORS);
+    if (column >= vectors) return;
+    const float *const o = a.part_o + 4 * ((item * (D / 4) + f) * a.tile + column);
+    for (int n0 = 0; n0 < kMergeQuads; n0 += N) {
+      MergedRuns<N> r;
+      r.read(a.part_ml + 2 * (item * a.tile + column), o + (int64_t)4 * n0 * a.tile, ml_step, o_step, 4 * a.tile, 0, 1, it.nsplit);
 #pragma unroll
-      for (int n = 0; n < N; ++n)
-        if (n * TEAMS <= spare) finish(r[n], column + n * TEAMS);
+      for (int n = 0; n < N; ++n) finish(column, f + n0 + n, r.out[n], r.total);
     }
   }
 }
@@ -164,7 +164,7 @@ static hipError_t launch_d(const PagedLaunches &l, hipStream_t stream) {
   }
   if (l.bytes() > 0) {
     const int rows = few.B, few_per_row = (int)l.few_merges(), many_per_row = (int)l.many_merges();
-    auto merge = l.few.items == 0 ? paged_merge_kernel<D, kMergeVectors> : paged_merge_kernel<D, 1>;
+    auto merge = l.few.items == 0 ? paged_merge_kernel<D, kMergeQuads> : paged_merge_kernel<D, 2>;
     hipLaunchKernelGGL(merge, dim3((unsigned)rows * (few_per_row + many_per_row)), dim3(kMergeThreads), 0, stream, few, many,
                        rows * few_per_row, few_per_row, many_per_row);
   }

@@ -24,7 +24,7 @@
 // 46 %, the vector units 56 %, a quarter of that exponentials), 32 / 8 heads 0.51 to 0.54 (990 to 1040), 16 / 4 heads of 256
 // features 0.56 (950; 40 and 38 %, the rest waits for LDS and the block's barrier).  One row of 512 tokens and 2048
 // keys, 16 / 8 heads: 30 us with the merge, of which the rounds are 10, the way to the first (plan, queries, first keys) 5,
-// the records 3 to write and 6 to merge; 64 tiles fill a quarter of the CUs, so it has to be cut.
+// the records 3 to write and 5 to merge; 64 tiles fill a quarter of the CUs, so it has to be cut.
 #pragma once
 
 #include "paged_decode.h"
@@ -324,14 +324,16 @@ __device__ __forceinline__ void paged_chunk_item(const PagedArgs &a, int index, 
   for (int d = 0; d < S::DT; ++d)
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[d][r] = o[d][r] * mine + over[(16 * d + r) * 64] * theirs;
-  // o[d][r] is feature 32 d + 8 (r / 4) + 4 h + r % 4.
+  // o[d][r] is feature 32 d + 8 (r / 4) + 4 h + r % 4.  Records hold four features of the tile's vectors side by side: whole
+  // lines a store.
   if (it.nsplit > 1) {
     const int64_t record = (int64_t)index * COLS + 32 * wave + m;
+    float *const part = a.part_o + 4 * (((int64_t)index * (D / 4) + h) * COLS + 32 * wave + m);
 #pragma unroll
     for (int d = 0; d < S::DT; ++d)
 #pragma unroll
       for (int r = 0; r < 4; ++r)
-        *as_global(reinterpret_cast<f32x4 *>(a.part_o + record * D + 32 * d + 8 * r + 4 * h)) =
+        *as_global(reinterpret_cast<f32x4 *>(part + 4 * (8 * d + 2 * r) * COLS)) =
             f32x4{o[d][4 * r], o[d][4 * r + 1], o[d][4 * r + 2], o[d][4 * r + 3]};
     if (h == 0) *as_global(reinterpret_cast<f32x2 *>(a.part_ml + 2 * record)) = f32x2{best, sum};
   } else {
@@ -511,11 +513,12 @@ __device__ __forceinline__ void paged_chunk_item_wide(const PagedArgs &a, int in
 
   sum = pair_sum32(pair_sum16(sum));
   if (!there) return;
-  // o[d][i] is feature 16 d + 4 g + i.
+  // o[d][i] is feature 16 d + 4 g + i.  Records hold four features of the tile's vectors side by side: whole lines a store.
   if (it.nsplit > 1) {
     const int64_t record = (int64_t)index * COLS + 16 * wave + m;
+    float *const part = a.part_o + 4 * (((int64_t)index * (D / 4) + g) * COLS + 16 * wave + m);
 #pragma unroll
-    for (int d = 0; d < S::DT; ++d) *as_global(reinterpret_cast<f32x4 *>(a.part_o + record * D + 16 * d + 4 * g)) = o[d];
+    for (int d = 0; d < S::DT; ++d) *as_global(reinterpret_cast<f32x4 *>(part + 4 * 4 * d * COLS)) = o[d];
     if (g == 0) *as_global(reinterpret_cast<f32x2 *>(a.part_ml + 2 * record)) = f32x2{top, sum};
   } else {
     const float by = sum == 0.0f ? 0.0f : 1.0f / sum;
