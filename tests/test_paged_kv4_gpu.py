@@ -8,9 +8,9 @@ Tolerances.  Codes, scales, slots and positions are compared whole.  A normalise
 a step, 2^-8 of its value at most, plus the fp32 arithmetic in front of it (some 10 roundings and one rsqrt of 1 ulp,
 under 2^-19 of the row's largest value).  An attention output is a weighted mean of values whose weights sum to one: the
 output's rounding is at most 2^-8 |out|; weights rounded to bf16 are off by at most 2^-8 of themselves and move the
-mean by at most 2^-8 sum(w |v|), counted twice where the sum of the weights is taken before their rounding; the scores'
-arithmetic (sums of up to 256 products that keep 2^-17 of their largest term, below 8 here, then one exponential) adds
-a relative 2^-12 of the weights.  So |error| <= 2^-8 |out| + (2^-7 + 2^-11) sum(w |v|).
+mean by at most 2^-8 sum(w |v|), and by as much again where the sum of the weights is taken after their rounding; the
+scores' arithmetic (sums of up to 256 products that keep 2^-17 of their largest term, below 8 here, then one
+exponential) adds a relative 2^-12 of the weights.  So |error| <= 2^-8 |out| + (2^-7 + 2^-11) sum(w |v|).
 """
 
 import numpy as np

@@ -5,7 +5,7 @@ decode steps captured in a HIP graph, requests that end and give their pages to 
 
 Bounds.  The same tokens in other chunks pass the same weights; keys, values and weights of the softmax are
 rounded alike, but sums run in another order and the projections have other shapes, so hidden states differ by bf16
-roundings (2^-9 of a value, some tens of them a layer) and a key that such a difference moves over a border of the
+roundings (about 2^-9 of a value in the mean, some tens of them a layer) and a key that such a difference moves over a border of the
 4-bit grid by a whole step (up to a third of it; about one key in 50, each 2^-9 / 2^-3 of the way).  That is
 sqrt(1 / 50) / 6, 2.4 % of a row's keys in norm, and less in a mean over keys: logits within a relative L2 of 5e-2.
 Against the unmodified model with keys and values put through the same format the keys are rounded to bf16 before it

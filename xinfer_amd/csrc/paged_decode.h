@@ -15,9 +15,9 @@
 // (w - bf16(w)), at no further matrix work, which leaves 2^-16 of a weight; with more the rounding is up to 2^-8.
 //
 // What bounds it: memory where there is much to read (64 rows of 1605 to 16384 keys, 16 / 8 heads of 128 features: 637 MB
-// in 139 us, 4.6 TB/s; 8 rows of 55 to 13312 keys, 34 MB: 17.0 us, 4 of them the merge), the vector unit close behind (a
-// wave's group takes some 200 vector instructions, 64 conversions and 16 exponentials, 0.35 us of a CU each in the end),
-// and latency where there is little (one row of 1 to 64 keys 6.1 us, 1024 keys 10.5 with the merge).
+// in 139 us, 4.6 TB/s, the vector units at work 40 % of the time; 8 rows of 55 to 13312 keys, 34 MB: 17.0 us, 4 of them
+// the merge), and latency where there is little (one row of 1 to 64 keys 6.1 us, 1024 keys 10.5 with the merge).  A wave's
+// group takes some 200 vector instructions, 64 conversions and 16 exponentials: 16 waves on one CU 0.35 us a group.
 #pragma once
 
 #include "paged_mfma.h"

@@ -20,11 +20,12 @@
 // sum before; with 128 features it makes no difference).
 //
 // What bounds it: matrix and vector unit share a SIMD's issue, and two waves hide little more.  512 tokens in each of 8 rows
-// of 8192 keys, page size 64: 16 / 8 heads of 128 features 0.28 to 0.29 ms (930 TFLOP/s; of the clocks the matrix units work
-// 46 %, the vector units 56 %, a quarter of that exponentials), 32 / 8 heads 0.51 to 0.54 (990 to 1040), 16 / 4 heads of 256
-// features 0.56 (950; 40 and 38 %, the rest waits for LDS and the block's barrier).  One row of 512 tokens and 2048
-// keys, 16 / 8 heads: 30 us with the merge, of which the rounds are 10, the way to the first (plan, queries, first keys) 5,
-// the records 3 to write and 5 to merge; 64 tiles fill a quarter of the CUs, so it has to be cut.
+// of 8192 keys, page size 64: 16 / 8 heads of 128 features 0.28 to 0.29 ms (920 to 960 TFLOP/s; the matrix units work 47 %
+// of the time, the vector units 57 %, a quarter of that exponentials), 32 / 8 heads 0.51 to 0.54 (990 to 1040), 16 / 4 heads
+// of 256 features 0.53 to 0.57 (940 to 1010; 43 and 40 %, a fifth waits for LDS, loads and the block's barrier).  One row
+// of 512 tokens and 2048 keys, 16 / 8 heads: 29 to 30 us with the merge, of which the rounds are 10, the way to the first
+// (plan, queries, first keys) 5, the records 3 to write and 5 to merge; 64 tiles fill a quarter of the CUs, so it has to be
+// cut.
 #pragma once
 
 #include "paged_decode.h"
