@@ -243,12 +243,13 @@ typedef struct xinfer_kv4_cache {
 
 /* Pages, slots and positions of a step from the rows' lengths, on the device.
  * Row r held ceil(kv_before[r] / P) pages and is to hold ceil(kv_lengths[r] / P),
- * with its last query_lengths[r] tokens new.  free_pages is a ring: entries
- * counters[0] <= i < counters[1] (modulo ring_size) are free.  Growing rows take
- * pages from its head in row order into block_table [rows][table_width];
- * shrinking rows (an ended request has length 0) put theirs at its tail, for
- * later calls.  A row whose pages, with those of the rows before it, exceed the
- * free ones, or that does not fit its table row, keeps its pages and takes no part:
+ * with its last query_lengths[r] tokens new.  free_pages is a ring with a place
+ * for every page: entries counters[0] <= i < counters[1] (modulo ring_size) are
+ * free.  Growing rows take pages from its head in row order into block_table
+ * [rows][table_width]; shrinking rows (an ended request has length 0) put theirs
+ * at its tail, for later calls.  A row whose pages, with those of the rows before
+ * it, exceed the free ones, or that does not fit its table row, keeps its pages and
+ * takes no part:
  * lengths[0][r] (new tokens) is 0 and lengths[1][r] is kv_before[r]; otherwise
  * they are query_lengths[r] and kv_lengths[r].  positions and slots [rows][tokens]
  * are written whole: of token t < lengths[0][r] the position kv_lengths[r] -

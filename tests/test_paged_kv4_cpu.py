@@ -125,6 +125,9 @@ def test_attention_refusals_and_workspace(lib):
     assert decode == (64 + 1024) * 16 * 130 * 4
     assert call(view(8, 16, 1, 128), width=256, size=decode - 1) == call(view(8, 16, 1, 128), width=256, workspace=BASE + 8) == WORKSPACE
     assert size(view(8, 16, 512, 128), cache(), 256, 0) > decode
+    # Records are those of cut rows, which are fewer than twice the items aimed at, whatever the batch.
+    assert size(view(64, 16, 8192, 128), cache(), 1024, 0) <= 2 * (768 * 128 + 256 * 32) * 130 * 4
+    assert size(view(4096, 16, 1, 128), cache(), 1024, 0) <= 2 * 1024 * 16 * 130 * 4
 
 
 def test_operators_check_their_tensors(library_path):

@@ -485,3 +485,69 @@ def test_a_cache_past_32_bits(ops):
         outs = [ops.paged_attention_kv4(q, c, torch.tensor([t], dtype=torch.int32, device="cuda"), state, 0, 0.1)
                 for c, t in ((big, places), (small, [0, 1, 2]))]
         assert torch.equal(*outs) and outs[0].any()
+
+
+def test_operators_refuse(ops):
+    """What the kernels do not serve is refused before a launch."""
+    log("paged kv4 refusals")
+    half = dict(dtype=torch.bfloat16, device="cuda")
+    cache = ops.paged_kv4_cache(4, 8, 64, 128, "cuda")
+    key, slots = torch.zeros(2, 8, 3, 128, **half), torch.zeros(2, 3, dtype=torch.int64, device="cuda")
+    q, table = torch.zeros(2, 16, 3, 128, **half), torch.zeros(2, 2, dtype=torch.int32, device="cuda")
+    rows = torch.tensor([[3, 3], [3, 3]], dtype=torch.int32, device="cuda")
+
+    def refused(message, call, *args):
+        with pytest.raises(RuntimeError, match=message):
+            call(*args)
+
+    refused("BF16", ops.append_kv4, key.half(), key.half(), slots, cache)
+    refused("inference only", ops.append_kv4, key.clone().requires_grad_(), key, slots, cache)
+    refused("int64 slots", ops.append_kv4, key, key, slots.int(), cache)
+    refused("int64 slots", ops.append_kv4, key, key, slots[:, :2], cache)
+    refused("colocated", ops.append_kv4, key, key, slots.cpu(), cache)
+    refused("uint8 cache", ops.append_kv4, key, key, slots, [t.int() for t in cache])
+    refused("uint8 cache", ops.read_kv4, [t[:, ::2] for t in cache], slots)
+    refused("cache codes", ops.append_kv4, key, key, slots, (cache[0], cache[1][..., :32].contiguous(), *cache[2:]))
+    refused("Tensors do not match", ops.append_kv4, key[..., :64], key[..., :64], slots, cache)
+    by_token, weight = key.transpose(1, 2), torch.ones(128, **half)
+    for width, message in ((24, "Tensors do not match"), (144, "Tensors do not match")):
+        turn = torch.ones(2, 3, width, **half)
+        refused(message, ops.qk_norm_rope_append_kv4, q.transpose(1, 2), by_token, by_token, weight, weight, 1e-6, 0.0, turn,
+                turn, slots, cache)
+    turn = torch.ones(2, 3, 64, **half)
+    refused("inference only", ops.qk_norm_rope_append_kv4, q.transpose(1, 2).requires_grad_(), by_token, by_token, weight,
+            weight, 1e-6, 0.0, turn, turn, slots, cache)
+    refused("inference only", ops.paged_attention_kv4, q.clone().requires_grad_(), cache, table, rows, 0, 0.1)
+    refused("block table", ops.paged_attention_kv4, q, cache, table.t(), rows, 0, 0.1)
+    refused("int32 lengths", ops.paged_attention_kv4, q, cache, table, rows.long(), 0, 0.1)
+    refused("scale", ops.paged_attention_kv4, q, cache, table, rows, 0, float("nan"))
+    refused("pages", ops.paged_attention_kv4, q, cache, table, rows, -1, 0.1)
+    refused("heads", ops.paged_attention_kv4, q[:, :12], cache, table, rows, 0, 0.1)
+    ring, counters = ops.free_page_ring(4, "cuda")
+    one = torch.zeros(2, dtype=torch.int32, device="cuda")
+    refused("pages", ops.paged_kv_reserve, one, one, one, 1, 96, counters, table, ring)
+    refused("row lengths", ops.paged_kv_reserve, one, one[:1], one, 1, 64, counters, table, ring)
+    refused("counters", ops.paged_kv_reserve, one, one, one, 1, 64, counters.int(), table, ring)
+    assert not any(t.any() for t in cache)
+
+
+def test_tensors_on_two_streams(ops):
+    """Calls of two streams at once, each with a workspace of its own, give what they give alone."""
+    log("paged_attention_kv4 two streams")
+    g = torch.Generator().manual_seed(14)
+    lengths = [3000, 2500]
+    table, pages = make_table(g, lengths, 64)
+    cache, t = filled_cache(ops, g, pages, 8, 64, 128), table.cuda()
+    work = []
+    for tokens in (1, 60):
+        q = randn(g, 2, 16, tokens, 128).cuda()
+        rows = torch.tensor([[tokens] * 2, lengths], dtype=torch.int32, device="cuda")
+        work.append((q, rows, ops.paged_attention_kv4(q, cache, t, rows, 0, 0.1), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for _ in range(3):
+        outs = []
+        for q, rows, _, stream in work:
+            with torch.cuda.stream(stream):
+                outs.append(ops.paged_attention_kv4(q, cache, t, rows, 0, 0.1))
+        torch.cuda.synchronize()
+        assert all(torch.equal(out, want) for out, (_, _, want, _) in zip(outs, work))

@@ -64,7 +64,7 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // cut, as the merge's launch costs more than it saves.
 PagedLaunch paged_launch(const PagedArgs &shapes, int vectors_min, int vectors_max, int tile, int min_groups, int target,
                          int whole_groups) {
-  PagedLaunch l{shapes, 0, 0, 0, 8};
+  PagedLaunch l{shapes, 0, 0, 0, 0, 8};
   l.a.vectors_min = vectors_min;
   l.a.vectors_max = vectors_max;
   l.a.tile = tile;
@@ -75,7 +75,9 @@ PagedLaunch paged_launch(const PagedArgs &shapes, int vectors_min, int vectors_m
   const int64_t runs = groups <= whole_groups ? 1 : ceil_div(groups, min_groups);
   l.a.min_groups = runs <= 1 ? (int)std::max<int64_t>(groups, 1) : min_groups;
   l.items = runs <= 1 ? whole : std::min(whole * runs, whole + target);
-  l.bytes = runs <= 1 ? 0 : (size_t)l.items * tile * (shapes.cache.D + 2) * sizeof(float);
+  // A row is cut where it has more groups than a run, so its items are fewer than twice its share of the target.
+  l.records = runs <= 1 ? 0 : std::min(l.items, 2 * (int64_t)target);
+  l.bytes = (size_t)l.records * tile * (shapes.cache.D + 2) * sizeof(float);
   return l;
 }
 
@@ -130,14 +132,14 @@ int paged_call(const xinfer_view4 &q, const xinfer_kv4_cache &cache, int64_t tab
   a.width = (int32_t)table_width;
   a.max_length = (int32_t)(max_length == 0 ? capacity : std::min(max_length, capacity));
   const int columns = paged_decode_columns(a.cache.D), vectors = a.T * a.G;
-  call.many = PagedLaunch{a, 0, 0, 0, 8};
+  call.many = PagedLaunch{a, 0, 0, 0, 0, 8};
   if (vectors <= 32) {
     call.few = paged_decode_launch(a, 32, vectors <= 16 ? 16 : columns, true);
     return paged_launchable(call);
   }
   // Rows of more vectors than a decode item has go to the prefill kernel; one row alone does whatever its count.
   const bool alone = B == 1;
-  call.few = alone ? PagedLaunch{a, 0, 0, 0, 8} : paged_decode_launch(a, columns, columns, false);
+  call.few = alone ? PagedLaunch{a, 0, 0, 0, 0, 8} : paged_decode_launch(a, columns, columns, false);
   call.many = paged_launch(a, alone ? 0 : columns + 1, kIntMax, kPagedPrefillTile, 8, alone || B > 64 ? kPagedCus : 3 * kPagedCus, 8);
   if (!alone) {
     // A record of 128 vectors is written and read at some 5 TB/s; a group of an item takes about 2 us.
@@ -283,7 +285,7 @@ int xinfer_paged_attention_kv4(const xinfer_view4 *q, const xinfer_kv4_cache *ca
     l->a.out = static_cast<uint16_t *>(out);
     l->a.scale_log2 = (float)(scale * 1.4426950408889634);
     l->a.part_o = reinterpret_cast<float *>(records);
-    l->a.part_ml = l->a.part_o + l->items * l->a.tile * l->a.cache.D;
+    l->a.part_ml = l->a.part_o + l->records * l->a.tile * l->a.cache.D;
     records += l->bytes;
   }
   return done(launch_paged_attention(call, static_cast<hipStream_t>(stream)));

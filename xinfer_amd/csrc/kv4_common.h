@@ -92,10 +92,11 @@ struct PagedArgs {
 // allow any, to the prefill kernel.
 struct PagedLaunch {
   PagedArgs a;
-  int64_t items;  // of the plan, at most: blocks, and records; 0: no launch
-  int tiles;      // of a row and KV head, at most
-  size_t bytes;   // of the records; 0: no row can be cut
-  int waves;      // of a decode block
+  int64_t items;    // of the plan, at most; 0: no launch
+  int64_t records;  // of cut rows' items, at most; 0: no row can be cut
+  int tiles;        // of a row and KV head, at most
+  size_t bytes;     // of the records
+  int waves;        // of a decode block
 };
 constexpr int kMergeThreads = 256, kMergeQuads = 4;  // of a merge block; quads of features a thread takes of a prefill row
 struct PagedLaunches {

@@ -67,6 +67,12 @@ void check_bf16(Tensors tensors) {
     TORCH_CHECK(t->scalar_type() == at::kBFloat16, "xinfer paged KV cache requires BF16 activations and weights");
 }
 
+// Weights may ask for gradients, as a model's do outside of training.
+void check_inference(Tensors activations) {
+  for (const at::Tensor *t : activations)
+    TORCH_CHECK(!t->requires_grad(), "xinfer paged KV cache supports inference only");
+}
+
 xinfer_kv4_cache cache_of(const at::Tensor &key, const at::Tensor &key_scale, const at::Tensor &value,
                           const at::Tensor &value_scale) {
   bool fine = true;
@@ -124,6 +130,7 @@ void append_kv4(const at::Tensor &key, const at::Tensor &value, const at::Tensor
   check_colocated(key, {&value, &slots, &key_codes, &key_scales, &value_codes, &value_scales});
   TORCH_CHECK(key.dim() == 4 && value.sizes() == key.sizes(), "Expected key/value [B,Hkv,T,D]");
   check_bf16({&key, &value});
+  check_inference({&key, &value});
   check_slots(slots, key.size(0), key.size(2));
   const auto cache = cache_of(key_codes, key_scales, value_codes, value_scales);
   c10::DeviceGuard guard(key.device());
@@ -160,6 +167,7 @@ at::Tensor qk_norm_rope_append_kv4(const at::Tensor &q, const at::Tensor &key, c
                   q_weight.size(0) == q.size(3) && k_weight.sizes() == q_weight.sizes(),
               "Expected q [B,T,Hq,D], key/value [B,T,Hkv,D], cos/sin [B,T,R] and [D] weights");
   check_bf16({&q, &key, &value, &q_weight, &k_weight, &cos, &sin});
+  check_inference({&q, &key, &value});
   check_slots(slots, q.size(0), q.size(1));
   const auto cache = cache_of(key_codes, key_scales, value_codes, value_scales);
   c10::DeviceGuard guard(q.device());

@@ -10,13 +10,14 @@ template <int D, int NC, int WAVES>
 __global__ void __launch_bounds__(64 * WAVES, D == 256 || NC == 2 ? 2 : 4) paged_decode_kernel(const PagedArgs a) {
   __shared__ __attribute__((aligned(1024))) char smem[kPagedDecodeLds<D, WAVES>];
   PagedItem it;
-  if (paged_item(a, paged_lane_row(a, 0), blockIdx.x, it)) paged_decode_item<D, NC, WAVES>(a, blockIdx.x, it, smem);
+  int index = blockIdx.x;
+  if (paged_item(a, paged_lane_row(a, 0), index, it)) paged_decode_item<D, NC, WAVES>(a, it, smem);
 }
 
 template <int D>
-__device__ __forceinline__ void paged_prefill_item(const PagedArgs &a, int index, const PagedItem &it, char *smem) {
-  if constexpr (D == 256) paged_chunk_item_wide<D>(a, index, it, smem);
-  else paged_chunk_item<D>(a, index, it, smem);
+__device__ __forceinline__ void paged_prefill_item(const PagedArgs &a, const PagedItem &it, char *smem) {
+  if constexpr (D == 256) paged_chunk_item_wide<D>(a, it, smem);
+  else paged_chunk_item<D>(a, it, smem);
 }
 
 // Prefill items first, the much shorter decode items behind them, where they fill what the last prefill items leave idle,
@@ -30,10 +31,9 @@ __global__ void __launch_bounds__(64 * kPagedChunkWaves, 2) paged_both_kernel(co
   int index = blockIdx.x;
   const PagedRow lane_row = paged_lane_row(many, 0);
   if (paged_item(many, lane_row, index, it)) {
-    paged_prefill_item<D>(many, index, it, smem);
-  } else {
-    index -= it.begin;
-    if (paged_item(few, lane_row, index, it)) paged_decode_item<D, paged_decode_columns(D) / 16, WAVES>(few, index, it, smem);
+    paged_prefill_item<D>(many, it, smem);
+  } else if (paged_item(few, lane_row, index, it)) {
+    paged_decode_item<D, paged_decode_columns(D) / 16, WAVES>(few, it, smem);
   }
 }
 
@@ -42,7 +42,8 @@ template <int D>
 __global__ void __launch_bounds__(64 * kPagedChunkWaves, 2) paged_prefill_kernel(const PagedArgs a) {
   __shared__ __attribute__((aligned(1024))) char smem[kPagedChunkLds<D>];
   PagedItem it;
-  if (paged_item(a, paged_lane_row(a, 0), blockIdx.x, it)) paged_prefill_item<D>(a, blockIdx.x, it, smem);
+  int index = blockIdx.x;
+  if (paged_item(a, paged_lane_row(a, 0), index, it)) paged_prefill_item<D>(a, it, smem);
 }
 
 // The running maximum, sum and output (N times four features) of a vector's runs so far.
@@ -106,7 +107,7 @@ __global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(const PagedA
   paged_row_items(a, row, it);
   if (it.nsplit <= 1 || tile >= it.tiles) return;
   const int vectors = min(it.count * a.G - tile * a.tile, a.tile);
-  const int64_t item = (int64_t)it.begin + (int64_t)tile * it.nsplit * a.cache.Hkv + h;
+  const int64_t item = (int64_t)it.record + (int64_t)tile * it.nsplit * a.cache.Hkv + h;
   const int64_t ml_step = 2 * (int64_t)a.cache.Hkv * a.tile, o_step = (int64_t)a.cache.Hkv * a.tile * D;
   // Output of four features from 4 f on.
   auto finish = [&](int column, int f, const f32x4 &sum, float total) {

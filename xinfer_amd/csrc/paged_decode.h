@@ -213,9 +213,9 @@ __device__ __forceinline__ void paged_scores(const GroupLoads<D> &in, const Quer
 template <int D, int WAVES>
 constexpr int kPagedDecodeLds = WAVES * (PagedShape<D>::STAGE + 16 * 8);
 
-// Item `it` of the plan, its `index`th, by the whole block; smem: kPagedDecodeLds bytes, 1024-byte aligned.
+// Item `it` of the plan, by the whole block; smem: kPagedDecodeLds bytes, 1024-byte aligned.
 template <int D, int NC, int WAVES>
-__device__ __forceinline__ void paged_decode_item(const PagedArgs &a, int index, const PagedItem &it, char *smem) {
+__device__ __forceinline__ void paged_decode_item(const PagedArgs &a, const PagedItem &it, char *smem) {
   using S = PagedShape<D>;
   constexpr int COLS = 16 * NC, THREADS = 64 * WAVES;
   f32x2 *const wave_ml = reinterpret_cast<f32x2 *>(smem + WAVES * S::STAGE);
@@ -386,7 +386,7 @@ __device__ __forceinline__ void paged_decode_item(const PagedArgs &a, int index,
         out += *reinterpret_cast<const f32x4 *>(smem + w * S::STAGE + column * (4 * D) + (f ^ (column & 7)) * 16) * keep;
       }
       if (it.nsplit > 1) {
-        const int64_t record = (int64_t)index * COLS + 16 * n + column;
+        const int64_t record = (int64_t)it.record * COLS + 16 * n + column;
         *as_global(reinterpret_cast<f32x4 *>(a.part_o + record * D + 4 * f)) = out;
         if (f == 0) *as_global(reinterpret_cast<f32x2 *>(a.part_ml + 2 * record)) = f32x2{best, total};
       } else {

@@ -37,7 +37,7 @@ struct PagedItem {
   int row, count, length;
   int h, tile, split, nsplit, tiles;
   int group_begin, group_end;  // 64-key groups of the run
-  int begin;                   // the row's first item
+  int record;                  // of cut rows' items, which are counted apart: this one's
 };
 
 // What a launch takes of row r: 64-key groups and tiles; no tiles: the row is another launch's.
@@ -111,31 +111,31 @@ __device__ __forceinline__ int paged_run(const PagedArgs &a, const PagedRows &fi
   return __builtin_amdgcn_readlane(run, __builtin_ctzll(__ballot(cost == best)));
 }
 
-// What lane `at` holds of its row; upto: items up to and with it.
-__device__ __forceinline__ void paged_take(PagedItem &it, const PagedRows &rows, int nsplit, int upto, int items, int at) {
+// What lane `at` holds of its row.
+__device__ __forceinline__ void paged_take(PagedItem &it, const PagedRows &rows, int nsplit, int at) {
   it.count = __builtin_amdgcn_readlane(rows.p.count, at);
   it.length = __builtin_amdgcn_readlane(rows.p.length, at);
   it.nsplit = __builtin_amdgcn_readlane(nsplit, at);
   it.tiles = __builtin_amdgcn_readlane(rows.s.tiles, at);
-  it.begin = __builtin_amdgcn_readlane(upto - items, at);
   it.group_end = __builtin_amdgcn_readlane(rows.s.groups, at);
 }
 
-// Item `index` of the plan; false past its last, it.begin is then how many there are.  Every lane of a wave calls it, with
-// the same index and its row of the first 64.
-__device__ __forceinline__ bool paged_item(const PagedArgs &a, const PagedRow &lane_row, int index, PagedItem &it) {
+// Item `index` of the plan, false past its last, index then goes down by how many there are.  Every lane of a wave calls it, with the same index and its row of the first 64.
+__device__ __forceinline__ bool paged_item(const PagedArgs &a, const PagedRow &lane_row, int &index, PagedItem &it) {
   const int Hkv = a.cache.Hkv;
   PagedRows rows;
   rows.take(a, 0, lane_row);
   const int run = paged_run(a, rows);
-  for (int base = 0, before = 0;;) {
-    const int nsplit = paged_splits(rows.s, run), items = rows.s.tiles * nsplit * Hkv, upto = before + wave_scan(items);
+  for (int base = 0, records = 0;;) {
+    const int nsplit = paged_splits(rows.s, run), items = rows.s.tiles * nsplit * Hkv, cut = nsplit > 1 ? items : 0;
+    const int upto = wave_scan(items), cut_upto = wave_scan(cut);
     const uint64_t past = __ballot(upto > index);
     if (past != 0) {
       const int at = __builtin_ctzll(past);
       it.row = base + at;
-      paged_take(it, rows, nsplit, upto, items, at);
-      const uint32_t i = index - it.begin, rest = i / (uint32_t)Hkv;
+      paged_take(it, rows, nsplit, at);
+      const uint32_t i = index - __builtin_amdgcn_readlane(upto - items, at), rest = i / (uint32_t)Hkv;
+      it.record = records + __builtin_amdgcn_readlane(cut_upto - cut, at) + (int)i;
       it.h = i - rest * Hkv;
       it.tile = rest / (uint32_t)it.nsplit;
       it.split = rest - it.tile * it.nsplit;
@@ -145,30 +145,29 @@ __device__ __forceinline__ bool paged_item(const PagedArgs &a, const PagedRow &l
       it.group_end = it.group_begin + each + (it.split < more ? 1 : 0);
       return true;
     }
+    index -= __builtin_amdgcn_readlane(upto, 63);
+    records += __builtin_amdgcn_readlane(cut_upto, 63);
     base += 64;
-    before = __builtin_amdgcn_readlane(upto, 63);
-    if (base >= a.B) {
-      it.begin = before;
-      return false;
-    }
+    if (base >= a.B) return false;
     rows.load(a, base);
   }
 }
 
-// Row `row`'s part of the plan: its first item, splits and tiles.
+// Row `row`'s part of the plan: its first record, splits and tiles.
 __device__ __forceinline__ void paged_row_items(const PagedArgs &a, int row, PagedItem &it) {
   PagedRows rows;
   rows.load(a, 0);
   const int run = paged_run(a, rows);
-  for (int base = 0, before = 0;; rows.load(a, base)) {
-    const int nsplit = paged_splits(rows.s, run), items = rows.s.tiles * nsplit * a.cache.Hkv, upto = before + wave_scan(items);
+  for (int base = 0, records = 0;; rows.load(a, base)) {
+    const int nsplit = paged_splits(rows.s, run), cut = nsplit > 1 ? rows.s.tiles * nsplit * a.cache.Hkv : 0, upto = wave_scan(cut);
     if (row < base + 64) {
       it.row = row;
-      paged_take(it, rows, nsplit, upto, items, row - base);
+      paged_take(it, rows, nsplit, row - base);
+      it.record = records + __builtin_amdgcn_readlane(upto - cut, row - base);
       return;
     }
     base += 64;
-    before = __builtin_amdgcn_readlane(upto, 63);
+    records += __builtin_amdgcn_readlane(upto, 63);
   }
 }
 

@@ -65,9 +65,9 @@ __device__ __forceinline__ void staged_barrier() { asm volatile("s_waitcnt lgkmc
 template <int D>
 constexpr int kPagedChunkLds = D == 256 ? 3 * 64 * 2 * D : 4 * 64 * 2 * D + kPagedPrefillTile * (2 * D + D / 32);
 
-// Item `it` of the plan, its `index`th, by the whole block; smem: kPagedChunkLds bytes, 1024-byte aligned.
+// Item `it` of the plan, by the whole block; smem: kPagedChunkLds bytes, 1024-byte aligned.
 template <int D>
-__device__ __forceinline__ void paged_chunk_item(const PagedArgs &a, int index, const PagedItem &it, char *smem) {
+__device__ __forceinline__ void paged_chunk_item(const PagedArgs &a, const PagedItem &it, char *smem) {
   using S = ChunkShape<D>;
   constexpr int COLS = 32 * kChunkWaves;
   const int tid = threadIdx.x & (kChunkThreads - 1), lane = tid & 63, m = lane & 31, h = lane >> 5;
@@ -328,8 +328,8 @@ __device__ __forceinline__ void paged_chunk_item(const PagedArgs &a, int index, 
   // o[d][r] is feature 32 d + 8 (r / 4) + 4 h + r % 4.  Records hold four features of the tile's vectors side by side: whole
   // lines a store.
   if (it.nsplit > 1) {
-    const int64_t record = (int64_t)index * COLS + 32 * wave + m;
-    float *const part = a.part_o + 4 * (((int64_t)index * (D / 4) + h) * COLS + 32 * wave + m);
+    const int64_t record = (int64_t)it.record * COLS + 32 * wave + m;
+    float *const part = a.part_o + 4 * (((int64_t)it.record * (D / 4) + h) * COLS + 32 * wave + m);
 #pragma unroll
     for (int d = 0; d < S::DT; ++d)
 #pragma unroll
@@ -351,7 +351,7 @@ __device__ __forceinline__ void paged_chunk_item(const PagedArgs &a, int index, 
 
 // The same for 256 features: 8 waves of 16 query vectors.
 template <int D>
-__device__ __forceinline__ void paged_chunk_item_wide(const PagedArgs &a, int index, const PagedItem &it, char *smem) {
+__device__ __forceinline__ void paged_chunk_item_wide(const PagedArgs &a, const PagedItem &it, char *smem) {
   using S = PagedShape<D>;
   constexpr int WAVES = kPagedChunkWaves, THREADS = 64 * WAVES, COLS = 16 * WAVES, BLOCKS = D / 32, STAGE = 64 * S::ROW;
   static_assert(64 * BLOCKS == THREADS, "a thread stages one block of one key");
@@ -516,8 +516,8 @@ __device__ __forceinline__ void paged_chunk_item_wide(const PagedArgs &a, int in
   if (!there) return;
   // o[d][i] is feature 16 d + 4 g + i.  Records hold four features of the tile's vectors side by side: whole lines a store.
   if (it.nsplit > 1) {
-    const int64_t record = (int64_t)index * COLS + 16 * wave + m;
-    float *const part = a.part_o + 4 * (((int64_t)index * (D / 4) + g) * COLS + 16 * wave + m);
+    const int64_t record = (int64_t)it.record * COLS + 16 * wave + m;
+    float *const part = a.part_o + 4 * (((int64_t)it.record * (D / 4) + g) * COLS + 16 * wave + m);
 #pragma unroll
     for (int d = 0; d < S::DT; ++d) *as_global(reinterpret_cast<f32x4 *>(part + 4 * 4 * d * COLS)) = o[d];
     if (g == 0) *as_global(reinterpret_cast<f32x2 *>(a.part_ml + 2 * record)) = f32x2{top, sum};

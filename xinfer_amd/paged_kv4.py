@@ -90,8 +90,9 @@ def paged_kv_reserve(kv_before, kv_lengths, query_lengths, tokens, page_size, co
     ``kv_before``, ``kv_lengths``, ``query_lengths``: int32 [B] on the device: each row's length before the step (what
     its pages were reserved for), after it, and how many of those are new (the last ones); ``tokens``: T, the padded
     number of new tokens.  A row may shrink (an ended request goes to 0, drafted tokens are taken back) and then gives
-    pages back, which serve from the next call on.  ``block_table`` int32 [B,M] and the ring ``free_pages`` are updated
-    in place; ``counters`` int64 [2], the ring's head and tail, is returned updated as a new tensor.
+    pages back, which serve from the next call on.  ``block_table`` int32 [B,M] and the ring ``free_pages`` (a place for
+    every page) are updated in place; ``counters`` int64 [2], the ring's head and tail, is returned updated as a new
+    tensor.
 
     ``lengths`` holds each row's real new tokens and its length: those asked for, or 0 and the length before for a row
     whose pages were not to be had.  Slots of padded tokens are -1, their positions 0.  The call gives the same again
