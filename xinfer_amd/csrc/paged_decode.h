@@ -83,10 +83,14 @@ struct GroupLoads {
     const int size = 1 << a.cache.page_shift;
     const int64_t head = (int64_t)page * a.cache.Hkv + h;
     const uint8_t *const codes = a.cache.key + (head * size + at) * (D / 2);
-    const uint8_t *const scales = a.cache.key_scale + head * (D / 32) * size + at;
 #pragma unroll
     for (int i = 0; i < S::KL; ++i)
       k[i] = *as_global(reinterpret_cast<const u32x4 *>(codes + (i / S::KC) * (D / 2) + (i % S::KC) * 64 + key_at));
+    key_scales(a, page, h, at);
+  }
+  __device__ __forceinline__ void key_scales(const PagedArgs &a, int page, int h, int at) {
+    const int size = 1 << a.cache.page_shift;
+    const uint8_t *const scales = a.cache.key_scale + ((int64_t)page * a.cache.Hkv + h) * (D / 32) * size + at;
 #pragma unroll
     for (int c = 0; c < S::KC; ++c)
       ks[c] = *as_global(reinterpret_cast<const uint32_t *>(scales + 4 * c * size + key_scale_at));

@@ -63,7 +63,7 @@ __device__ __forceinline__ void staged_barrier() { asm volatile("s_waitcnt lgkmc
 // LDS of a prefill block: staged groups, two for each half of the waves, and the queries' terms and scales, later the
 // second half's maxima and sums (256 features: three groups for all waves).
 template <int D>
-constexpr int kPagedChunkLds = D == 256 ? 3 * 64 * 2 * D : 4 * 64 * 2 * D + kPagedPrefillTile * (2 * D + D / 32);
+constexpr int kPagedChunkLds = D == 256 ? 3 * 64 * (2 * D + D / 2) : 4 * 64 * 2 * D + kPagedPrefillTile * (2 * D + D / 32);
 
 // Item `it` of the plan, by the whole block; smem: kPagedChunkLds bytes, 1024-byte aligned.
 template <int D>
@@ -353,7 +353,7 @@ __device__ __forceinline__ void paged_chunk_item(const PagedArgs &a, const Paged
 template <int D>
 __device__ __forceinline__ void paged_chunk_item_wide(const PagedArgs &a, const PagedItem &it, char *smem) {
   using S = PagedShape<D>;
-  constexpr int WAVES = kPagedChunkWaves, THREADS = 64 * WAVES, COLS = 16 * WAVES, BLOCKS = D / 32, STAGE = 64 * S::ROW;
+  constexpr int WAVES = kPagedChunkWaves, THREADS = 64 * WAVES, COLS = 16 * WAVES, BLOCKS = D / 32, STAGE = 64 * S::ROW, KEYS = 64 * (D / 2);
   static_assert(64 * BLOCKS == THREADS, "a thread stages one block of one key");
   const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -408,15 +408,30 @@ __device__ __forceinline__ void paged_chunk_item_wide(const PagedArgs &a, const 
       *(__attribute__((address_space(3))) u32x4 *)((put_at ^ (16 * c)) + buffer * STAGE) = kv4_values(v[c], scale);
   };
 
+  // Keys are staged too, as they are: from the lanes' own rows a load would take one clock for 16 bytes of each lane, and
+  // every wave would read all of them.  Chunk c of key r lies at c ^ (r / 4): a lane reads keys 4 m + t.
+  const uint32_t keys = stage + 3 * STAGE, put_key_at = keys + key * (D / 2) + (block ^ ((key >> 2) & 7)) * 16;
+  uint32_t get_key_at = keys + 4 * m * (D / 2) + (g ^ (m & 7)) * 16;
+  auto load_codes = [&](int group, int page) {
+    const int64_t hd = (int64_t)max(page, 0) * a.cache.Hkv + it.h;
+    return *as_global(reinterpret_cast<const u32x4 *>(a.cache.key + (hd * size + place(group)) * (D / 2) + 16 * tid));
+  };
+  auto put_codes = [&](int buffer, const u32x4 &codes) {
+    *(__attribute__((address_space(3))) u32x4 *)(put_key_at + buffer * KEYS) = codes;
+  };
   GroupLoads<D> in;
   in.init(size, stage, m, g);
   f32x4 s[4];
   uint32_t pw[2][4];
-  // A group's scores, then the loads of the next one's keys.
-  auto scores = [&](int next, int next_page) {
+  // A group's scores, then the loads of the next one's scales.
+  auto scores = [&](int buffer, int next, int next_page) {
+    const uint32_t get = get_key_at + buffer * KEYS;
+#pragma unroll
+    for (int i = 0; i < S::KL; ++i)
+      in.k[i] = *(const __attribute__((address_space(3))) u32x4 *)((get ^ (64 * (i % S::KC))) + (i / S::KC) * (D / 2));
     paged_scores<D>(in, q, g, s);
     asm volatile("" : "+v"(s[0]), "+v"(s[1]), "+v"(s[2]), "+v"(s[3]) : : "memory");
-    in.keys(a, max(next_page, 0), it.h, place(next));
+    in.key_scales(a, max(next_page, 0), it.h, place(next));
   };
   // Weights of a group: s[t][i] is key 16 g + 4 i + t.
   auto weights = [&](int group, int page) {
@@ -470,36 +485,43 @@ __device__ __forceinline__ void paged_chunk_item_wide(const PagedArgs &a, const 
   // Waves w and w + 4 share a SIMD.  Between two barriers the first half of the waves computes weights, then the
   // matrix products (this group's output, the next one's scores); the second half the products first (the last
   // group's output, this one's scores), then weights: one's matrix work runs beside the other's vector work.  So three
-  // groups' values are staged: the last, this and the next one.
+  // groups' values are staged: the last, this and the next one, and the keys of this and the two next.
   // Each half has a loop of its own: in a common one the compiler's waits for loads would be those of either order.
   const int begin = it.group_begin;
   auto sweep = [&](auto order) {
     constexpr bool AHEAD = decltype(order)::value;
-    int page = page_of(begin), next_page = page_of(begin + 1);
+    int page = page_of(begin), next_page = page_of(begin + 1), after_page = page_of(begin + 2);
     load_values(begin, page);
-    in.keys(a, max(page, 0), it.h, place(begin));
+    u32x4 codes = load_codes(begin, page), next_codes = load_codes(begin + 1, next_page);
+    in.key_scales(a, max(page, 0), it.h, place(begin));
     q.convert(qx, m, g);
     put_values(0);
+    put_codes(0, codes);
+    put_codes(1, next_codes);
     load_values(begin + 1, next_page);
-    if constexpr (AHEAD) scores(begin + 1, next_page);
+    codes = load_codes(begin + 2, after_page);
+    staged_barrier();
+    if constexpr (AHEAD) scores(0, begin + 1, next_page);
     int last = 2, now = 0, next = 1;  // staged groups' buffers
     for (int group = begin; group < group_end; ++group) {
-      asm volatile("" : "+v"(in.key_at), "+v"(in.key_scale_at), "+v"(get_at));
-      const int after_page = page_of(group + 2);
+      asm volatile("" : "+v"(in.key_scale_at), "+v"(get_at), "+v"(get_key_at));
+      const int far_page = page_of(group + 3);
       const bool active = group * kGroupKeys < none_see;  // uniform in the wave
-      staged_barrier();  // every wave has stored its part of this group's values
+      staged_barrier();  // every wave has stored its part of this group's values and of the next one's keys
       if constexpr (!AHEAD) {
         if (group > begin && (group - 1) * kGroupKeys < none_see) output(last);
-        scores(group + 1, next_page);
+        scores(now, group + 1, next_page);
       }
       put_values(next);
+      put_codes(last, codes);
       load_values(group + 2, after_page);
+      codes = load_codes(group + 3, far_page);
       if (active) weights(group, page);
       if constexpr (AHEAD) {
         if (active) output(now);
-        scores(group + 2, after_page);
+        scores(next, group + 2, after_page);
       }
-      page = next_page, next_page = after_page;
+      page = next_page, next_page = after_page, after_page = far_page;
       const int free = last;
       last = now, now = next, next = free;
     }
