@@ -380,10 +380,9 @@ __device__ __forceinline__ void paged_chunk_item_wide(const PagedArgs &a, const 
   const int shift = a.cache.page_shift - 6, size = 1 << a.cache.page_shift;
   typedef const __attribute__((address_space(4))) int32_t *table_ptr;
   const table_ptr table = (table_ptr)(a.table + (int64_t)it.row * a.width);
-  auto page_of = [&](int group) {
-    const int page = group < group_end ? table[group >> shift] : -1;
-    return page >= 0 && page < a.cache.pages ? page : -1;
-  };
+  auto entry_of = [&](int group) { return group < group_end ? table[group >> shift] : -1; };
+  auto checked = [&](int page) { return page >= 0 && page < a.cache.pages ? page : -1; };
+  auto page_of = [&](int group) { return checked(entry_of(group)); };
   auto place = [&](int group) { return (group & ((1 << shift) - 1)) * kGroupKeys; };
 
   // Staged values: 16-byte chunk c of key r lies at slot c ^ S(r) ^ (c / 8), which puts the eight blocks of a key that eight
@@ -469,7 +468,7 @@ __device__ __forceinline__ void paged_chunk_item_wide(const PagedArgs &a, const 
   auto output = [&](int buffer) {
     const uint32_t get = get_at + buffer * STAGE;
     __builtin_amdgcn_s_setprio(1);  // before the other wave's vector work (5 chunks, 3 single tokens: 395 us, without 407)
-    pipelined<2 * S::DT, 4>(
+    pipelined<2 * S::DT, 8>(
         [&](int k) {
           const int u = k / S::DT, d = k % S::DT;
           const uint32_t at = (get ^ (32 * d) ^ (16 * (d >> 2))) + 8 * u * S::ROW;
@@ -490,7 +489,7 @@ __device__ __forceinline__ void paged_chunk_item_wide(const PagedArgs &a, const 
   const int begin = it.group_begin;
   auto sweep = [&](auto order) {
     constexpr bool AHEAD = decltype(order)::value;
-    int page = page_of(begin), next_page = page_of(begin + 1), after_page = page_of(begin + 2);
+    int page = page_of(begin), next_page = page_of(begin + 1), after_page = page_of(begin + 2), far_page = page_of(begin + 3);
     load_values(begin, page);
     u32x4 codes = load_codes(begin, page), next_codes = load_codes(begin + 1, next_page);
     in.key_scales(a, max(page, 0), it.h, place(begin));
@@ -505,7 +504,7 @@ __device__ __forceinline__ void paged_chunk_item_wide(const PagedArgs &a, const 
     int last = 2, now = 0, next = 1;  // staged groups' buffers
     for (int group = begin; group < group_end; ++group) {
       asm volatile("" : "+v"(in.key_scale_at), "+v"(get_at), "+v"(get_key_at));
-      const int far_page = page_of(group + 3);
+      const int far_entry = entry_of(group + 4);  // looked at when it has arrived, at the end
       const bool active = group * kGroupKeys < none_see;  // uniform in the wave
       staged_barrier();  // every wave has stored its part of this group's values and of the next one's keys
       if constexpr (!AHEAD) {
@@ -521,7 +520,7 @@ __device__ __forceinline__ void paged_chunk_item_wide(const PagedArgs &a, const 
         if (active) output(now);
         scores(next, group + 2, after_page);
       }
-      page = next_page, next_page = after_page, after_page = far_page;
+      page = next_page, next_page = after_page, after_page = far_page, far_page = checked(far_entry);
       const int free = last;
       last = now, now = next, next = free;
     }
