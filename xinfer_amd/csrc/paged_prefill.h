@@ -63,7 +63,7 @@ __device__ __forceinline__ void staged_barrier() { asm volatile("s_waitcnt lgkmc
 // LDS of a prefill block: staged groups, two for each half of the waves, and the queries' terms and scales, later the
 // second half's maxima and sums (256 features: three groups for all waves).
 template <int D>
-constexpr int kPagedChunkLds = D == 256 ? 3 * 64 * (2 * D + D / 2) : 4 * 64 * 2 * D + kPagedPrefillTile * (2 * D + D / 32);
+constexpr int kPagedChunkLds = D == 256 ? 3 * (64 * 2 * D + 65 * (D / 2)) : 4 * 64 * 2 * D + kPagedPrefillTile * (2 * D + D / 32);
 
 // Item `it` of the plan, by the whole block; smem: kPagedChunkLds bytes, 1024-byte aligned.
 template <int D>
@@ -353,7 +353,7 @@ __device__ __forceinline__ void paged_chunk_item(const PagedArgs &a, const Paged
 template <int D>
 __device__ __forceinline__ void paged_chunk_item_wide(const PagedArgs &a, const PagedItem &it, char *smem) {
   using S = PagedShape<D>;
-  constexpr int WAVES = kPagedChunkWaves, THREADS = 64 * WAVES, COLS = 16 * WAVES, BLOCKS = D / 32, STAGE = 64 * S::ROW, KEYS = 64 * (D / 2);
+  constexpr int WAVES = kPagedChunkWaves, THREADS = 64 * WAVES, COLS = 16 * WAVES, BLOCKS = D / 32, STAGE = 64 * S::ROW, KEYS = 65 * (D / 2);
   static_assert(64 * BLOCKS == THREADS, "a thread stages one block of one key");
   const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -408,9 +408,11 @@ __device__ __forceinline__ void paged_chunk_item_wide(const PagedArgs &a, const 
   };
 
   // Keys are staged too, as they are: from the lanes' own rows a load would take one clock for 16 bytes of each lane, and
-  // every wave would read all of them.  Chunk c of key r lies at c ^ (r / 4): a lane reads keys 4 m + t.
-  const uint32_t keys = stage + 3 * STAGE, put_key_at = keys + key * (D / 2) + (block ^ ((key >> 2) & 7)) * 16;
-  uint32_t get_key_at = keys + 4 * m * (D / 2) + (g ^ (m & 7)) * 16;
+  // every wave would read all of them.  Chunk c of key r lies at c ^ (r / 4)
+  // of row r + r / 32: a lane reads keys 4 m + t, and 16 lanes' reads fill even and odd rows.
+  const uint32_t keys = stage + 3 * STAGE;
+  const uint32_t put_key_at = keys + (key + (key >> 5)) * (D / 2) + (block ^ ((key >> 2) & 7)) * 16;
+  uint32_t get_key_at = keys + (4 * m + (m >> 3)) * (D / 2) + (g ^ (m & 7)) * 16;
   auto load_codes = [&](int group, int page) {
     const int64_t hd = (int64_t)max(page, 0) * a.cache.Hkv + it.h;
     return *as_global(reinterpret_cast<const u32x4 *>(a.cache.key + (hd * size + place(group)) * (D / 2) + 16 * tid));
