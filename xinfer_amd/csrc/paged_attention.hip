@@ -22,7 +22,7 @@ __device__ __forceinline__ void paged_prefill_item(const PagedArgs &a, const Pag
 
 // Prefill items first, the much shorter decode items behind them, where they fill what the last prefill items leave idle,
 // then the blocks without an item.  (A batch of 5 chunks and 3 single tokens, 256 features: 432 us, with the decode
-// items first 447; 390 now.)
+// items first 447; 368 now.)
 template <int D>
 __global__ void __launch_bounds__(64 * kPagedChunkWaves, 2) paged_both_kernel(const PagedArgs few, const PagedArgs many) {
   constexpr int WAVES = kPagedChunkWaves, CHUNK = kPagedChunkLds<D>, DECODE = kPagedDecodeLds<D, WAVES>;

@@ -75,7 +75,7 @@ __device__ __forceinline__ int paged_splits(const PagedShare &s, int run) { retu
 // eight: n items of at most m groups on kPagedSlots blocks at a time take no longer than ceil(n / slots) m, nor than
 // their mean load and m; an item costs kPagedItemGroups more (queries in, output out) and a record what it is written
 // and read for (a.record_groups).  On a batch of 5 rows of 33 to 223 groups, 256 features: 432 us with targets up to
-// 768, 499 with 512 or 256 (390 now); uniform batches choose 256 (4 rows of 64 groups, 128 features: 94 us, with 256 alone 92, the rest
+// 768, 499 with 512 or 256 (368 now); uniform batches choose 256 (4 rows of 64 groups, 128 features: 94 us, with 256 alone 92, the rest
 // being blocks without an item).
 constexpr int kPagedSlots = 256;
 constexpr float kPagedItemGroups = 4.0f;

@@ -22,7 +22,7 @@
 // What bounds it: matrix and vector unit share a SIMD's issue, and two waves hide little more.  512 tokens in each of 8 rows
 // of 8192 keys, page size 64: 16 / 8 heads of 128 features 0.28 to 0.29 ms (920 to 960 TFLOP/s; the matrix units work 47 %
 // of the time, the vector units 57 %, a quarter of that exponentials), 32 / 8 heads 0.51 to 0.54 (990 to 1040), 16 / 4 heads
-// of 256 features 0.53 to 0.57 (940 to 1010; 43 and 40 %, a fifth waits for LDS, loads and the block's barrier).  One row
+// of 256 features 0.50 to 0.52 (1020 to 1060; 46 and 43 %, LDS 36 %, and waits for it and the block's barrier).  One row
 // of 512 tokens and 2048 keys, 16 / 8 heads: 29 to 30 us with the merge, of which the rounds are 10, the way to the first
 // (plan, queries, first keys) 5, the records 3 to write and 5 to merge; 64 tiles fill a quarter of the CUs, so it has to be
 // cut.
@@ -408,7 +408,8 @@ __device__ __forceinline__ void paged_chunk_item_wide(const PagedArgs &a, const 
   };
 
   // Keys are staged too, as they are: from the lanes' own rows a load would take one clock for 16 bytes of each lane, and
-  // every wave would read all of them.  Chunk c of key r lies at c ^ (r / 4)
+  // every wave would read all of them (5 chunks, 3 single tokens: 370 us, 390 so; with 128 features, where half as many
+  // loads a product do it, staging cost 4 %).  Chunk c of key r lies at c ^ (r / 4)
   // of row r + r / 32: a lane reads keys 4 m + t, and 16 lanes' reads fill even and odd rows.
   const uint32_t keys = stage + 3 * STAGE;
   const uint32_t put_key_at = keys + (key + (key >> 5)) * (D / 2) + (block ^ ((key >> 2) & 7)) * 16;
@@ -469,7 +470,7 @@ __device__ __forceinline__ void paged_chunk_item_wide(const PagedArgs &a, const 
   };
   auto output = [&](int buffer) {
     const uint32_t get = get_at + buffer * STAGE;
-    __builtin_amdgcn_s_setprio(1);  // before the other wave's vector work (5 chunks, 3 single tokens: 395 us, without 407)
+    __builtin_amdgcn_s_setprio(1);  // before the other wave's vector work (5 chunks, 3 single tokens: 395 us, 407 without)
     pipelined<2 * S::DT, 8>(
         [&](int k) {
           const int u = k / S::DT, d = k % S::DT;
